@@ -296,6 +296,72 @@ mhip_status mhip_greedy_select_f32(mhip_ctx* ctx, const float* logits, uint64_t 
 mhip_status mhip_kv_write_f32(mhip_ctx* ctx, float* store, uint64_t capacity, uint64_t width,
                               const float* rows, uint64_t count, uint64_t row_offset);
 
+/* ---- 4-bit KV stores (no counterpart in the reference) ----
+ * A store holds the f32 rows [capacity, kv_heads * head_dimension] of a key or
+ * value cache in 4 bits a value: each block of 32 values of a head (the last
+ * one filled up with zeros) as E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) under one power of two, 17/32 of a byte a value. A value x of a
+ * block is held as code * 2^e: e the smallest exponent under which the block's
+ * largest magnitude rounds to at most 6 (from -120 to 125), the code the
+ * nearest to x / 2^e, ties to the even one. A block with a value that is not
+ * finite is held as 32 NaN. The same shape goes with every call on a store. */
+typedef struct {
+    uint64_t capacity;          /* rows, below 2^31 - 512 */
+    uint64_t kv_heads;
+    uint64_t head_dimension;    /* 1 .. 256 */
+    uint64_t batch;             /* stores of this shape, one a sequence (0: 1) */
+    uint64_t batch_stride;      /* bytes between them, a multiple of 16
+                                   (0: mhip_kv_mx4_bytes) */
+} mhip_mx4_store;
+/* Bytes of one store (a multiple of 256; 0 for a shape that is refused). The
+ * buffer is 16-byte aligned; zeroed, it holds zeros. */
+uint64_t mhip_kv_mx4_bytes(uint64_t capacity, uint64_t kv_heads, uint64_t head_dimension);
+/* kv-write: rows [batch][count, kv_heads * head_dimension] into each store's
+ * rows [row_offset, row_offset + count); other rows unchanged. An overrun is
+ * ShapeUnsupported and writes nothing. Advances as mhip_kv_write_f32 does. */
+mhip_status mhip_kv_write_mx4(mhip_ctx* ctx, void* store, const mhip_mx4_store* shape,
+                              const float* rows, uint64_t count, uint64_t row_offset);
+/* The values that rows [row_offset, row_offset + count) of each store hold,
+ * to rows [batch][count, kv_heads * head_dimension]. */
+mhip_status mhip_kv_read_mx4(mhip_ctx* ctx, const void* store, const mhip_mx4_store* shape,
+                             float* rows, uint64_t count, uint64_t row_offset);
+/* mhip_attention_f32 over a key and a value store of kv_rows rows: the same
+ * parameters and semantics (value_dimension 0 or head_dimension; kv_batch_stride
+ * and v_batch_stride are bytes, as mhip_mx4_store.batch_stride). With weights_out
+ * [batch][kv_head_count][kv_rows], also the attention that each key received:
+ * weights_out = weights + the sum, over the queries and the query heads of the
+ * KV head, of the softmax weight given to the key, for the kv_seq_len keys in
+ * use; entries past them stay as they are. weights has the same layout, NULL
+ * counts as zeros, and may be weights_out itself. */
+mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const void* k_store,
+                               const void* v_store, float* out,
+                               const mhip_attention_params* params, const float* weights,
+                               float* weights_out);
+/* Eviction by accumulated attention: of the key_count rows in use, each head of
+ * each sequence keeps the `first` first, the `recent` last and, of the rows
+ * between, those of the largest weights (ties to the lowest row; NaN counts as
+ * -inf, -0 as 0), `keep` rows in all. They become rows 0 .. keep - 1 of the
+ * output stores in their order, codes and scales as they were; rows from keep
+ * on stay as they are. weights [batch][kv_heads][weight_stride] (0: the
+ * capacity), weights_out likewise over the output shape's capacity, its entries
+ * from keep on 0 (what the rows written next start from), indices
+ * [batch][kv_heads][keep]: the kept rows' former numbers (NULL: not wanted).
+ * The output stores are either others or, both, the stores themselves (the
+ * same shape); so are the weights. Nothing advances in a captured step. */
+typedef struct {
+    uint64_t key_count;
+    uint64_t keep;
+    uint64_t first;
+    uint64_t recent;
+    uint64_t weight_stride;
+    uint64_t weight_out_stride;
+} mhip_kv_evict_params;
+mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, const void* v_store,
+                              const float* weights, const mhip_mx4_store* shape,
+                              const mhip_kv_evict_params* params, void* k_out, void* v_out,
+                              const mhip_mx4_store* out_shape, float* weights_out,
+                              uint32_t* indices);
+
 /* ---- step capture and replay (src/kernels.rs:1019-1349, src/executor.rs:177-336) ----
  * Between mhip_capture_begin and mhip_capture_end, the context's launches are
  * recorded (kernel, grid, argument values) instead of running; a replay

@@ -105,6 +105,19 @@ class AttentionParams(ctypes.Structure):
     ]
 
 
+class Mx4StoreShape(ctypes.Structure):
+    """mhip_mx4_store: the shape of a 4-bit KV store."""
+    _fields_ = [("capacity", ctypes.c_uint64), ("kv_heads", ctypes.c_uint64),
+                ("head_dimension", ctypes.c_uint64), ("batch", ctypes.c_uint64),
+                ("batch_stride", ctypes.c_uint64)]
+
+
+class KvEvictParams(ctypes.Structure):
+    _fields_ = [("key_count", ctypes.c_uint64), ("keep", ctypes.c_uint64),
+                ("first", ctypes.c_uint64), ("recent", ctypes.c_uint64),
+                ("weight_stride", ctypes.c_uint64), ("weight_out_stride", ctypes.c_uint64)]
+
+
 _P = ctypes.c_void_p
 _U64 = ctypes.c_uint64
 _F = ctypes.c_float
@@ -156,6 +169,13 @@ SIGNATURES = {
     "mhip_embedding_bf16w_f32": [_CTX, _P, _U64, _U64, _P, _U64, _P],
     "mhip_greedy_select_f32": [_CTX, _P, _U64, _U64, _U64, _P, ctypes.c_uint32, ctypes.c_float,
                                ctypes.POINTER(ctypes.c_int64)],
+    "mhip_kv_mx4_bytes": [_U64, _U64, _U64],
+    "mhip_kv_write_mx4": [_CTX, _P, ctypes.POINTER(Mx4StoreShape), _P, _U64, _U64],
+    "mhip_kv_read_mx4": [_CTX, _P, ctypes.POINTER(Mx4StoreShape), _P, _U64, _U64],
+    "mhip_attention_mx4": [_CTX, _P, _P, _P, _P, ctypes.POINTER(AttentionParams), _P, _P],
+    "mhip_kv_evict_mx4": [_CTX, _P, _P, _P, ctypes.POINTER(Mx4StoreShape),
+                          ctypes.POINTER(KvEvictParams), _P, _P, ctypes.POINTER(Mx4StoreShape), _P,
+                          _P],
     "mhip_capture_begin": [_CTX, ctypes.c_uint32],
     "mhip_capture_end": [_CTX, ctypes.POINTER(_P), ctypes.POINTER(_U64)],
     "mhip_capture_abort": [_CTX],
@@ -171,6 +191,7 @@ _RESTYPES = {
     "mhip_version": ctypes.c_char_p,
     "mhip_rope_params_default": None,
     "mhip_graph_max_offset": _U64,
+    "mhip_kv_mx4_bytes": _U64,
 }
 
 _lib = None
