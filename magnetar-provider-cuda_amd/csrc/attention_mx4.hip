@@ -27,6 +27,12 @@
 //
 // so neither the weights nor the values pass through LDS, and a row's maximum
 // and its rescaling are its own lane's.
+//
+// Up to four rows (a token of up to four query heads a KV head) leave twelve of
+// the sixteen columns empty: there the planes take columns of their own, column
+// 4 * plane + row (the fourth plane is zero), and a product is one matrix
+// instruction instead of three. Scores are added up over the planes' lanes, the
+// outputs once at the end.
 #include <cmath>
 
 #include "mx4.hpp"
@@ -35,6 +41,7 @@ namespace {
 
 using mhip::bf16x2;
 using mhip::bf16x8;
+using mhip::f32x2;
 using mhip::f32x4;
 using mhip::Mx4Unit;
 
@@ -55,9 +62,12 @@ struct Mx4Attn {
     int vec;                      // rows of q and out are whole float4s
     int row_tiles, chunks;
     float c;                      // scale * log2(e)
-    float* part_o;                // [batch][kv head][row tile][chunk][16][DP]
-    float* part_ml;               // [batch][kv head][row tile][chunk][16][2]
+    float* part_o;                // [batch][kv head][row tile][chunk][row][DP]
+    float* part_ml;               // [batch][kv head][row tile][chunk][row][2]
+    uint32_t* arrived;            // [batch][kv head][row tile]: chunks done, 0 between calls
     float* stats;                 // [batch][kv head][rows][2]: m and 1 / l (weights asked for)
+    float* kept;                  // [batch][kv head][rows][kept_ld]: scores (weights asked for, one row tile)
+    uint64_t kept_ld;
 };
 
 // The keys [lo, hi) that a row's query admits, and those that all rows of a
@@ -107,11 +117,55 @@ __device__ __forceinline__ uint32_t bits(bf16x2 v) {
     return u;
 }
 
+// The plane that a lane of the few-rows form has: x less the part that the
+// planes before it hold. The masks of plane 3 leave x - x, zero.
+struct Plane {
+    uint32_t m1, m2;
+};
+__device__ __forceinline__ Plane plane_of(int slot) {
+    return Plane{slot == 0 ? 0u : slot == 3 ? 0xFFFFFFFFu : 0xFFFF0000u, slot == 2 ? 0xFFFF0000u : 0u};
+}
+__device__ __forceinline__ float plane_part(float x, Plane p) {
+    x -= __uint_as_float(__float_as_uint(x) & p.m1);
+    return x - __uint_as_float(__float_as_uint(x) & p.m2);
+}
+__device__ __forceinline__ void plane8(const float (&x)[8], Plane p, Frag& f) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y) f.u[y] = top16(plane_part(x[2 * y + 1], p), plane_part(x[2 * y], p));
+}
+
+// x summed over the lanes n, n + 4, n + 8 and n + 12 of 16.
+__device__ __forceinline__ float sum_planes(float x) {
+    x += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xF, 0xF, true));  // row_ror:8
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x124, 0xF, 0xF, true));  // row_ror:4
+}
+
+// The operand of a product's rows: FEW one plane a lane, else all three.
+template <bool FEW>
+struct Rows {
+    Frag f[FEW ? 1 : 3];
+};
+template <bool FEW>
+__device__ __forceinline__ void rows8(const float (&x)[8], Plane p, Rows<FEW>& w) {
+    if constexpr (FEW)
+        plane8(x, p, w.f[0]);
+    else
+        split8(x, w.f);
+}
+template <bool FEW>
+__device__ __forceinline__ f32x4 product(const Frag& a, const Rows<FEW>& w, f32x4 c) {
+    if constexpr (!FEW) {
+        c = mfma(a, w.f[2], c);
+        c = mfma(a, w.f[1], c);
+    }
+    return mfma(a, w.f[0], c);
+}
+
 // Row `row`'s part of Q for lane group g: step s, pair y takes byte x = 4 s + y
 // of the lane group's units in order (unit n = 4 t + g of t = x / NB, block p =
 // x % NB): columns 32 p + n and 32 p + 16 + n.
-template <int NB>
-__device__ __forceinline__ void load_q(const Mx4Attn& a, const float* qrow, int g, Frag (&q)[NB][3]) {
+template <int NB, bool FEW>
+__device__ __forceinline__ void load_q(const Mx4Attn& a, const float* qrow, int g, Plane plane, Rows<FEW> (&q)[NB]) {
 #pragma unroll
     for (int s = 0; s < NB; ++s) {
         float x[8];
@@ -119,10 +173,11 @@ __device__ __forceinline__ void load_q(const Mx4Attn& a, const float* qrow, int 
         for (int y = 0; y < 4; ++y) {
             const int t = (4 * s + y) / NB, p = (4 * s + y) % NB;
             const int col = 32 * p + 4 * t + g;
-            x[2 * y] = col < a.d ? qrow[col] : 0.0f;
-            x[2 * y + 1] = col + 16 < a.d ? qrow[col + 16] : 0.0f;
+            const float x0 = qrow[min(col, a.d - 1)], x1 = qrow[min(col + 16, a.d - 1)];
+            x[2 * y] = col < a.d ? x0 : 0.0f;
+            x[2 * y + 1] = col + 16 < a.d ? x1 : 0.0f;
         }
-        split8(x, q[s]);
+        rows8<FEW>(x, plane, q[s]);
     }
 }
 
@@ -151,9 +206,9 @@ __device__ __forceinline__ void load_v(const uint32_t* codes, const uint32_t* sc
     }
 }
 
-// S^T of 64 keys by 16 rows: st[i][r] is key 16 g + 4 r + i of row q.
-template <int NB>
-__device__ __forceinline__ void scores(const Strip<NB>& k, const Frag (&q)[NB][3], f32x4 (&st)[4]) {
+// S^T of 64 keys: st[i][r] is key 16 g + 4 r + i of the lane's row.
+template <int NB, bool FEW>
+__device__ __forceinline__ void scores(const Strip<NB>& k, const Rows<FEW> (&q)[NB], f32x4 (&st)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -165,24 +220,25 @@ __device__ __forceinline__ void scores(const Strip<NB>& k, const Frag (&q)[NB][3
                 const int t = (4 * s + y) / NB, p = (4 * s + y) % NB, at = i * NB + p;
                 f.u[y] = bits(mhip::mx4_bf16(k.unit[t].w[at / 4], mhip::mx4_scale(k.scale[0].w[p], i), at % 4));
             }
-            acc = mfma(f, q[s][2], acc);
-            acc = mfma(f, q[s][1], acc);
-            acc = mfma(f, q[s][0], acc);
+            acc = product<FEW>(f, q[s], acc);
         }
+        if constexpr (FEW)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = sum_planes(acc[r]);
         st[i] = acc;
     }
 }
 
 // O^T += V^T P^T over 64 keys, p as scores() left them.
-template <int NB>
-__device__ __forceinline__ void outputs(const Strip<NB>& v, const float (&p)[4][4], f32x4 (&o)[2 * NB]) {
+template <int NB, bool FEW>
+__device__ __forceinline__ void outputs(const Strip<NB>& v, const float (&p)[4][4], Plane plane, f32x4 (&o)[2 * NB]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // 32 keys: r = 2 u and 2 u + 1
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = p[j % 4][2 * u + j / 4];
-        Frag w[3];
-        split8(x, w);
+        Rows<FEW> w;
+        rows8<FEW>(x, plane, w);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             Frag lo, hi;  // columns 32 b + n and 32 b + 16 + n
@@ -194,11 +250,8 @@ __device__ __forceinline__ void outputs(const Strip<NB>& v, const float (&p)[4][
                 lo.u[y] = __builtin_amdgcn_perm(k1, k0, 0x05040100u);
                 hi.u[y] = __builtin_amdgcn_perm(k1, k0, 0x07060302u);
             }
-#pragma unroll
-            for (int plane = 2; plane >= 0; --plane) {
-                o[2 * b] = mfma(lo, w[plane], o[2 * b]);
-                o[2 * b + 1] = mfma(hi, w[plane], o[2 * b + 1]);
-            }
+            o[2 * b] = product<FEW>(lo, w, o[2 * b]);
+            o[2 * b + 1] = product<FEW>(hi, w, o[2 * b + 1]);
         }
     }
 }
@@ -209,45 +262,39 @@ __device__ __forceinline__ void outputs(const Strip<NB>& v, const float (&p)[4][
 // finite) and, for the rows that admit the key, put into the sums of its
 // columns. `base`: the strip's first key; keys from `hi` on belong to no row.
 template <int NB>
-__device__ __forceinline__ void edge_values(Strip<NB>& v, int base, int g, int lane, const Keys& row, int hi,
-                                            f32x4 (&o)[2 * NB]) {
-    uint32_t flags[4][NB];
+__device__ __forceinline__ void edge_values(Strip<NB>& v, int base, int g, const Keys& row, int hi, f32x4 (&o)[2 * NB]) {
+    uint32_t flags[NB];  // bit 4 r + i: the block of key 16 g + 4 r + i is no number
     uint32_t any = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int b = 0; b < NB; ++b) {
+        flags[b] = 0;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            flags[r][b] = 0;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t byte = 255u << (8 * i);
                 const bool nan = (v.scale[r].w[b] & byte) == byte;
                 const bool past = base + 16 * g + 4 * r + i >= hi;
                 if (nan || past) v.scale[r].w[b] &= ~byte;
-                if (nan && !past) flags[r][b] |= 1u << i;
+                if (nan && !past) flags[b] |= 1u << (4 * r + i);
             }
-            any |= flags[r][b];
-        }
+        any |= flags[b];
+    }
     if (__ballot(any != 0) == 0) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int b = 0; b < NB; ++b) {
+        bool hit = false;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t lanes = __ballot((flags[r][b] >> i & 1u) != 0);
-                if (lanes == 0) continue;
-                bool hit = false;
-#pragma unroll
-                for (int gg = 0; gg < 4; ++gg) {
-                    const int key = base + 16 * gg + 4 * r + i;
-                    if ((lanes >> (16 * gg) & 1u) && key >= row.lo && key < row.hi) hit = true;
-                }
-                if (hit) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[2 * b][e] = o[2 * b + 1][e] = NAN;
-                }
+        for (int gg = 0; gg < 4; ++gg)
+            for (uint32_t keys = __builtin_amdgcn_readlane(flags[b], 16 * gg); keys != 0; keys &= keys - 1) {
+                const int key = base + 16 * gg + __builtin_ctz(keys);
+                if (key >= row.lo && key < row.hi) hit = true;
             }
+        if (hit) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[2 * b][e] = o[2 * b + 1][e] = NAN;
+        }
+    }
 }
 
 // Row `row`'s place in q or out.
@@ -256,33 +303,82 @@ __device__ __forceinline__ uint64_t row_at(const Mx4Attn& a, int kvh, int row) {
     return static_cast<uint64_t>(i) * a.q_ld + static_cast<uint64_t>(head) * a.d;
 }
 
-constexpr int kWaves = 4;
+constexpr int kWeightWaves = 4;
+constexpr int kMaxChunks = 256;
+// Waves of a rows workgroup: eight, of a head of more than four blocks four
+// (their sums in LDS are 16 rows a wave).
+template <bool FEW>
+constexpr int kRowTile = FEW ? 4 : 16;
+template <int NB>
+constexpr int kRowWaves = NB > 4 ? 4 : 8;
 
-// A workgroup: 16 rows of a KV head over one chunk of their keys, the chunk's
+// One row's outputs for four columns.
+__device__ __forceinline__ void store_out(const Mx4Attn& a, int b, int kvh, int row, int col, f32x4 o) {
+    float* dst = a.out + b * a.o_bs + row_at(a, kvh, row) + col;
+    if (a.vec) {
+        if (col < a.d) *reinterpret_cast<f32x4*>(dst) = o;
+    } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (col + x < a.d) dst[x] = o[x];
+    }
+}
+
+// Chunk records pass between workgroups whose L2 caches differ. They go past
+// the caches, as stores and loads at device scope, 8 bytes each: a store is
+// done once vmcnt has counted it, and only then does its workgroup count itself
+// in. (Plain stores under a device fence took 100-140 us more with 512-1024
+// workgroups: every fence writes a whole L2 back.)
+__device__ __forceinline__ void put2(float* p, float x, float y) {
+    const uint64_t v = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 get2(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return f32x2{__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32))};
+}
+
+// A workgroup: 16 rows of a KV head (FEW: 4) over one chunk of their keys, the chunk's
 // 64-key strips dealt to the waves in turn, the waves' sums added up in LDS.
 // The chunks split the keys that the tile's rows admit evenly; how many there
 // are goes by the store's capacity, how long they are by the key count, which a
-// replay moves.
-template <int NB>
-__global__ __launch_bounds__(64 * kWaves) void mx4_rows_kernel(Mx4Attn a) {
-    constexpr int DP = 32 * NB;
-    __shared__ float lds_o[kWaves][16][DP + 4];
-    __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+// replay moves. Of several chunks the workgroup that ends last adds up the
+// records of all, in their order, each weighted by 2 to its maximum less the
+// largest: one launch, and the same bits whichever it is.
+//
+// The next strip's keys are loaded once the scores have taken this one's, its
+// values once the outputs have: both loads run under the other product, in the
+// registers that it has freed.
+template <int NB, bool FEW>
+__global__ __launch_bounds__(64 * kRowWaves<NB>) void mx4_rows_kernel(Mx4Attn a) {
+    constexpr int DP = 32 * NB, kWaves = kRowWaves<NB>, kThreads = 64 * kWaves, RT = kRowTile<FEW>;
+    union Lds {
+        struct {
+            float o[kWaves][RT][DP + 4];
+        } waves;
+        struct {
+            float factor[RT][kMaxChunks];
+            f32x4 sum[kThreads];
+            float l[RT];
+        } merge;
+    };
+    __shared__ Lds lds;
+    __shared__ float lds_m[kWaves][RT], lds_l[kWaves][RT];
+    __shared__ uint32_t lds_last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int chunk = blockIdx.x % a.chunks, tile = blockIdx.x / a.chunks;
+    const int chunk = a.chunks > 1 ? blockIdx.x % a.chunks : 0, tile = a.chunks > 1 ? blockIdx.x / a.chunks : blockIdx.x;
     const int kvh = blockIdx.y, b = blockIdx.z;
     const int kv = a.kv + (a.advance ? static_cast<int>(*a.advance) : 0);
 
-    const int row0 = tile * 16, row_last = min(row0 + 15, a.rows - 1);
-    const int row = min(row0 + n, row_last);
+    const int row0 = tile * RT, row_last = min(row0 + RT - 1, a.rows - 1), live = row_last - row0 + 1;
+    const int slot = n / RT, own = n % RT, row = min(row0 + own, row_last);
+    const Plane plane = plane_of(slot);
     const Keys mine = row_keys(a, kv, row), head = row_keys(a, kv, row0), tail = row_keys(a, kv, row_last);
     const int begin = head.lo / 64, end = (tail.hi + 63) / 64;  // strips
-    const int per = (end - begin + a.chunks - 1) / a.chunks;
+    const int per = a.chunks > 1 ? (end - begin + a.chunks - 1) / a.chunks : end - begin;
     const int s0 = begin + chunk * per, s1 = min(s0 + per, end);
 
-    Frag q[NB][3];
-    load_q<NB>(a, a.q + b * a.q_bs + row_at(a, kvh, row), g, q);
     const uint8_t* ks = a.k + b * a.k_bs;
     const uint8_t* vs = a.v + b * a.v_bs;
     const uint64_t head_units = static_cast<uint64_t>(kvh) * a.groups;
@@ -292,17 +388,28 @@ __global__ __launch_bounds__(64 * kWaves) void mx4_rows_kernel(Mx4Attn a) {
     const uint32_t* vx = reinterpret_cast<const uint32_t*>(vs + a.code_bytes) + head_units * NB;
     const int last = (kv - 1) / 4;
 
+    Strip<NB> k, v;
+    int s = s0 + wave;
+    load_k<NB>(kc, kx, s * 16, last, n, g, k);
+    load_v<NB>(vc, vx, s * 16, last, n, g, v);
+    Rows<FEW> q[NB];
+    load_q<NB, FEW>(a, a.q + b * a.q_bs + row_at(a, kvh, row), g, plane, q);
+
     f32x4 o[2 * NB];
 #pragma unroll
     for (int c = 0; c < 2 * NB; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    for (int s = s0 + wave; s < s1; s += kWaves) {
+    for (; s < s1; s += kWaves) {
         const int base = 64 * s;
-        Strip<NB> k, v;
-        load_k<NB>(kc, kx, base / 4, last, n, g, k);
-        load_v<NB>(vc, vx, base / 4, last, n, g, v);
         f32x4 st[4];
-        scores<NB>(k, q, st);
+        scores<NB, FEW>(k, q, st);
+        load_k<NB>(kc, kx, (s + kWaves) * 16, last, n, g, k);
+        if (a.kept && n < live) {
+            float* to = a.kept + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows + row) * a.kept_ld + base + 16 * g;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x4*>(to + 4 * r) = f32x4{st[0][r], st[1][r], st[2][r], st[3][r]};
+        }
         const bool edge = base < tail.lo || base + 64 > head.hi;
         if (edge) {
 #pragma unroll
@@ -312,7 +419,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx4_rows_kernel(Mx4Attn a) {
                     const int key = base + 16 * g + 4 * r + i;
                     if (key < mine.lo || key >= mine.hi) st[i][r] = -INFINITY;
                 }
-            edge_values<NB>(v, base, g, lane, mine, tail.hi, o);
+            edge_values<NB>(v, base, g, mine, tail.hi, o);
         }
         float top = -INFINITY;
 #pragma unroll
@@ -334,124 +441,200 @@ __global__ __launch_bounds__(64 * kWaves) void mx4_rows_kernel(Mx4Attn a) {
                 sum += p[i][r];
             }
         l = l * alpha + sum;
+        if (__ballot(alpha != 1.0f) != 0) {
 #pragma unroll
-        for (int c = 0; c < 2 * NB; ++c)
+            for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[c][e] *= alpha;
-        outputs<NB>(v, p, o);
+                for (int e = 0; e < 4; ++e) o[c][e] *= alpha;
+        }
+        outputs<NB, FEW>(v, p, plane, o);
+        load_v<NB>(vc, vx, (s + kWaves) * 16, last, n, g, v);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    if (g == 0) {
-        lds_m[wave][n] = m;
-        lds_l[wave][n] = l;
-    }
+    if (g == 0 && slot == 0) lds_m[wave][own] = m;
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, lds_m[w][n]);
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, lds_m[w][own]);
     const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
-    for (int c = 0; c < 2 * NB; ++c)
-        *reinterpret_cast<f32x4*>(&lds_o[wave][n][16 * c + 4 * g]) = o[c] * f;
-    if (g == 0) lds_l[wave][n] = l * f;
+    for (int c = 0; c < 2 * NB; ++c) {
+        if constexpr (FEW)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][e] = sum_planes(o[c][e]);
+        if (slot == 0) *reinterpret_cast<f32x4*>(&lds.waves.o[wave][own][16 * c + 4 * g]) = o[c] * f;
+    }
+    if (g == 0 && slot == 0) lds_l[wave][own] = l * f;
     __syncthreads();
 
     const uint64_t tile_id = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.row_tiles + tile;
     const uint64_t rec = tile_id * a.chunks + chunk;
-    for (int e = threadIdx.x; e < 16 * DP / 4; e += 64 * kWaves) {
-        const int r = e / (DP / 4), col = e % (DP / 4) * 4;
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        float total = 0.0f;
+    if (a.chunks > 1) {
+        // Two columns a lane: a wave's stores fill whole lines.
+        for (int e = threadIdx.x; e < live * (DP / 2); e += kThreads) {
+            const int r = e / (DP / 2), col = e % (DP / 2) * 2;
+            f32x2 sum = {0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            sum += *reinterpret_cast<const f32x4*>(&lds_o[w][r][col]);
-            total += lds_l[w][r];
+            for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x2*>(&lds.waves.o[w][r][col]);
+            put2(a.part_o + (rec * RT + r) * DP + col, sum.x, sum.y);
         }
-        if (a.chunks > 1) {
-            *reinterpret_cast<f32x4*>(a.part_o + (rec * 16 + r) * DP + col) = sum;
-            continue;
-        }
-        if (row0 + r >= a.rows) continue;
-        const float inv = 1.0f / total;
-        float* dst = a.out + b * a.o_bs + row_at(a, kvh, row0 + r) + col;
-        if (a.vec) {
-            if (col < a.d) *reinterpret_cast<f32x4*>(dst) = sum * inv;
-        } else {
+    } else {
+        for (int e = threadIdx.x; e < live * (DP / 4); e += kThreads) {
+            const int r = e / (DP / 4), col = e % (DP / 4) * 4;
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            float total = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (col + x < a.d) dst[x] = sum[x] * inv;
+            for (int w = 0; w < kWaves; ++w) {
+                sum += *reinterpret_cast<const f32x4*>(&lds.waves.o[w][r][col]);
+                total += lds_l[w][r];
+            }
+            store_out(a, b, kvh, row0 + r, col, sum * (1.0f / total));
         }
     }
-    if (threadIdx.x < 16) {
+    if (threadIdx.x < live) {
         float total = 0.0f, mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            total += lds_l[w][n];
-            mx = fmaxf(mx, lds_m[w][n]);
+            total += lds_l[w][threadIdx.x];
+            mx = fmaxf(mx, lds_m[w][threadIdx.x]);
         }
         if (a.chunks > 1) {
-            a.part_ml[(rec * 16 + n) * 2] = mx;
-            a.part_ml[(rec * 16 + n) * 2 + 1] = total;
-        } else if (a.stats && row0 + n < a.rows) {
-            float* st = a.stats + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows + row0 + n) * 2;
+            put2(a.part_ml + (rec * RT + threadIdx.x) * 2, mx, total);
+        } else if (a.stats) {
+            float* st = a.stats + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows + row0 + threadIdx.x) * 2;
             st[0] = mx == -INFINITY ? 0.0f : mx;
             st[1] = 1.0f / total;
         }
     }
+    if (a.chunks == 1) return;
+
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) lds_last = atomicInc(&a.arrived[tile_id], a.chunks - 1) == static_cast<uint32_t>(a.chunks) - 1;
+    __syncthreads();
+    if (!lds_last) return;
+
+    // Four columns a thread; where those are few, `ways` threads share a cell's
+    // chunks. The first records are on their way while the rows' maxima are found.
+    constexpr int kAhead = 8;
+    const int cells = live * (DP / 4);
+    int ways = 1;
+    while (ways * 2 * cells <= kThreads) ways *= 2;
+    const float* records = a.part_o + tile_id * a.chunks * RT * DP;
+    auto record = [&](int cell, int c) {
+        const float* at = records + static_cast<uint64_t>(c) * RT * DP + cell * 4;
+        const f32x2 x = get2(at), y = get2(at + 2);
+        return f32x4{x.x, x.y, y.x, y.y};
+    };
+    const int cell0 = static_cast<int>(threadIdx.x) % cells, way = static_cast<int>(threadIdx.x) / cells;
+    f32x4 ahead[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const int c = way + j * ways;
+        ahead[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (way < ways && c < a.chunks) ahead[j] = record(cell0, c);
+    }
+    // kThreads / RT threads a row, at most a wave.
+    {
+        constexpr int kPer = kThreads / RT < 64 ? kThreads / RT : 64, kOwn = kMaxChunks / kPer;
+        const int r = threadIdx.x / kPer, c0 = threadIdx.x % kPer;
+        const float* ml = a.part_ml + (tile_id * a.chunks * RT + r) * 2;
+        f32x2 rec_ml[kOwn];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            const int c = c0 + j * kPer;
+            rec_ml[j] = f32x2{-INFINITY, 0.0f};
+            if (r < live && c < a.chunks) rec_ml[j] = get2(ml + c * 2 * RT);
+        }
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) mx = fmaxf(mx, rec_ml[j].x);
+#pragma unroll
+        for (int off = 1; off < kPer; off *= 2) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+        const float m_use = mx == -INFINITY ? 0.0f : mx;
+        float total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            const int c = c0 + j * kPer;
+            const float fc = __builtin_amdgcn_exp2f(rec_ml[j].x - m_use);
+            if (r < live && c < a.chunks) lds.merge.factor[r][c] = fc;
+            total += rec_ml[j].y * fc;
+        }
+#pragma unroll
+        for (int off = 1; off < kPer; off *= 2) total += __shfl_xor(total, off, 64);
+        if (r < live && c0 == 0) {
+            lds.merge.l[r] = 1.0f / total;
+            if (a.stats) {
+                float* st = a.stats + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows + row0 + r) * 2;
+                st[0] = m_use;
+                st[1] = 1.0f / total;
+            }
+        }
+    }
+    __syncthreads();
+    for (int cell = cell0; cell < cells; cell += kThreads) {  // more than one only where ways is 1
+        const int r = cell / (DP / 4), col = cell % (DP / 4) * 4;
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        int c = way;
+        if (cell == cell0) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j, c += ways)
+                if (way < ways && c < a.chunks) sum += ahead[j] * lds.merge.factor[r][c];
+        }
+        if (way < ways)
+#pragma unroll 4
+            for (; c < a.chunks; c += ways) sum += record(cell, c) * lds.merge.factor[r][c];
+        if (ways > 1) {
+            lds.merge.sum[threadIdx.x] = sum;
+            __syncthreads();
+            if (way == 0)
+                for (int w = 1; w < ways; ++w) sum += lds.merge.sum[w * cells + cell];
+        }
+        if (way == 0) store_out(a, b, kvh, row0 + r, col, sum * lds.merge.l[r]);
+    }
 }
 
-// The chunks' sums of one row: each weighted by 2 to its maximum less the
-// largest. A wave a row.
-template <int NB>
-__global__ __launch_bounds__(256) void mx4_merge_kernel(Mx4Attn a, uint64_t total_rows) {
-    constexpr int DP = 32 * NB;
-    const uint64_t id = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (id >= total_rows) return;
-    const int row = static_cast<int>(id % a.rows);
-    const uint64_t bh = id / a.rows;
-    const int kvh = static_cast<int>(bh % a.kv_heads), b = static_cast<int>(bh / a.kv_heads);
-    const uint64_t rec = (bh * a.row_tiles + row / 16) * a.chunks;
-    const int r = row % 16;
-    float top = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, a.part_ml[((rec + c) * 16 + r) * 2]);
+// The attention each key received, from the scores that the rows kernel kept
+// (one row tile): weights_out = weights + the sum over the rows of p. Four keys
+// a thread.
+__global__ __launch_bounds__(256) void mx4_kept_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
+                                                               float* weights_out, uint64_t stride) {
+    const int kv = a.kv + (a.advance ? static_cast<int>(*a.advance) : 0);
+    const int key = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (key >= kv) return;
+    const uint64_t bh = static_cast<uint64_t>(blockIdx.z) * a.kv_heads + blockIdx.y;
+    const float* st = a.stats + bh * a.rows * 2;
+    float sum[4] = {};
+    for (int row = 0; row < a.rows; ++row) {
+        const Keys in = row_keys(a, kv, row);
+        if (key + 3 < in.lo || key >= in.hi) continue;
+        const f32x4 s = *reinterpret_cast<const f32x4*>(a.kept + (bh * a.rows + row) * a.kept_ld + key);
+        const float m = st[2 * row], inv = st[2 * row + 1];
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const float m = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
-    float o[(DP + 63) / 64] = {};
-    for (int c = 0; c < a.chunks; ++c) {
-        const uint64_t at = (rec + c) * 16 + r;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
-        l += a.part_ml[2 * at + 1] * f;
-#pragma unroll
-        for (int x = 0; x < (DP + 63) / 64; ++x)
-            if (lane + 64 * x < DP) o[x] += a.part_o[at * DP + lane + 64 * x] * f;
+        for (int x = 0; x < 4; ++x) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], a.c, -m)) * inv;
+            if (key + x >= in.lo && key + x < in.hi) sum[x] += p;
+        }
     }
-    const float inv = 1.0f / l;
-    float* dst = a.out + b * a.o_bs + row_at(a, kvh, row);
+    const uint64_t at = bh * stride + key;
 #pragma unroll
-    for (int x = 0; x < (DP + 63) / 64; ++x)
-        if (lane + 64 * x < a.d) dst[lane + 64 * x] = o[x] * inv;
-    if (a.stats && lane == 0) {
-        a.stats[id * 2] = m;
-        a.stats[id * 2 + 1] = inv;
-    }
+    for (int x = 0; x < 4; ++x)
+        if (key + x < kv) weights_out[at + x] = (weights ? weights[at + x] : 0.0f) + sum[x];
 }
 
-// The attention each key received: weights_out = weights + the sum over a KV
-// head's rows of p, from the rows' statistics and the scores taken again. A
+// The same for any number of rows, the scores taken again from the rows'
+// statistics. A
 // wave takes 64 keys and every row tile that admits one of them.
 template <int NB>
-__global__ __launch_bounds__(64 * kWaves) void mx4_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
+__global__ __launch_bounds__(64 * kWeightWaves) void mx4_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
                                                                   float* weights_out, uint64_t stride) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.y, b = blockIdx.z;
     const int kv = a.kv + (a.advance ? static_cast<int>(*a.advance) : 0);
-    const int base = (blockIdx.x * kWaves + wave) * 64;
+    const int base = (blockIdx.x * kWeightWaves + wave) * 64;
     if (base >= kv) return;
     const uint8_t* ks = a.k + b * a.k_bs;
     const uint64_t head_units = static_cast<uint64_t>(kvh) * a.groups;
@@ -467,10 +650,10 @@ __global__ __launch_bounds__(64 * kWaves) void mx4_weights_kernel(Mx4Attn a, con
     const float* stats = a.stats + (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows * 2;
     for (int tile = i0 * a.group / 16; tile * 16 < i1 * a.group; ++tile) {
         const int row = min(tile * 16 + n, a.rows - 1);
-        Frag q[NB][3];
-        load_q<NB>(a, a.q + b * a.q_bs + row_at(a, kvh, row), g, q);
+        Rows<false> q[NB];
+        load_q<NB, false>(a, a.q + b * a.q_bs + row_at(a, kvh, row), g, Plane{}, q);
         f32x4 st[4];
-        scores<NB>(k, q, st);
+        scores<NB, false>(k, q, st);
         const Keys mine = row_keys(a, kv, row);
         const float m = stats[2 * row], inv = stats[2 * row + 1];
         const bool live = tile * 16 + n < a.rows;
@@ -501,42 +684,50 @@ __global__ __launch_bounds__(64 * kWaves) void mx4_weights_kernel(Mx4Attn a, con
     }
 }
 
-template <int NB>
+template <int NB, bool FEW>
 mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* weights, float* weights_out,
                         uint64_t stride, uint64_t kv_rows) {
+    a.row_tiles = static_cast<int>(mhip::ceil_div(a.rows, kRowTile<FEW>));
     const uint64_t tiles = batch * a.kv_heads * a.row_tiles;
-    // Enough workgroups for two on each CU, of at least two strips a wave.
-    uint64_t chunks = mhip::ceil_div(static_cast<uint64_t>(ctx->compute_units) * 2, tiles);
-    chunks = std::max<uint64_t>(1, std::min(chunks, mhip::ceil_div(kv_rows, 64 * kWaves)));
+    // A workgroup for each CU, of at least a strip a wave. (Two on each, with half
+    // the chunk: 8 x 4096 keys 19 us for 15, 131073 keys 42 for 33, what the
+    // waves' own part and the records cost more than what they hide.)
+    uint64_t chunks = mhip::ceil_div(ctx->compute_units, tiles);
+    chunks = std::min<uint64_t>({chunks, mhip::ceil_div(kv_rows, 64 * kRowWaves<NB>), kMaxChunks});
+    if (tiles > mhip::kMx4Counters) chunks = 1;
     a.chunks = static_cast<int>(chunks);
-    const uint64_t records = tiles * chunks * 16;
-    const uint64_t part_bytes = chunks > 1 ? records * (32 * NB + 2) * sizeof(float) : 0;
+    const uint64_t records = tiles * chunks * kRowTile<FEW>;
     const uint64_t total_rows = batch * a.kv_heads * static_cast<uint64_t>(a.rows);
-    const uint64_t bytes = part_bytes + (weights_out ? total_rows * 2 * sizeof(float) : 0);
+    if (a.row_tiles * chunks >= (1ULL << 31) || mhip::ceil_div(total_rows, 4) >= (1ULL << 31))
+        return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    const bool keep = weights_out && a.row_tiles == 1;
+    a.kept_ld = (kv_rows + 63) / 64 * 64;
+    const uint64_t part_bytes = chunks > 1 ? records * (32 * NB + 2) * sizeof(float) : 0;
+    const uint64_t kept_bytes = keep ? total_rows * a.kept_ld * sizeof(float) : 0;
+    const uint64_t bytes = part_bytes + kept_bytes + (weights_out ? total_rows * 2 * sizeof(float) : 0);
     if (bytes) {
         void* ws = nullptr;
         mhip_status st = mhip::workspace(ctx, bytes, &ws);
         if (st != MHIP_OK) return st;
         a.part_o = static_cast<float*>(ws);
         a.part_ml = a.part_o + records * (32 * NB);
-        if (weights_out) a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part_bytes);
+        a.kept = keep ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part_bytes) : nullptr;
+        if (weights_out) a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part_bytes + kept_bytes);
     }
-    if (a.row_tiles * chunks >= (1ULL << 31) || mhip::ceil_div(total_rows, 4) >= (1ULL << 31))
-        return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    a.arrived = ctx->mx4_arrived;
     const dim3 grid(static_cast<unsigned>(a.row_tiles * chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
-    mhip::launch(ctx, mx4_rows_kernel<NB>, grid, dim3(64 * kWaves), 0, a);
+    mhip::launch(ctx, mx4_rows_kernel<NB, FEW>, grid, dim3(64 * kRowWaves<NB>), 0, a);
     mhip_status st = mhip::check_launch("attention (4-bit)");
-    if (st == MHIP_OK && chunks > 1) {
-        mhip::launch(ctx, mx4_merge_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(total_rows, 4))), dim3(256), 0, a, total_rows);
-        st = mhip::check_launch("attention (4-bit, merge)");
-    }
-    if (st == MHIP_OK && weights_out) {
-        const uint64_t keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
-        const dim3 wgrid(static_cast<unsigned>(mhip::ceil_div(keys, 64 * kWaves)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
-        mhip::launch(ctx, mx4_weights_kernel<NB>, wgrid, dim3(64 * kWaves), 0, a, weights, weights_out, stride);
-        st = mhip::check_launch("attention (4-bit, weights)");
-    }
-    return st;
+    if (st != MHIP_OK || !weights_out) return st;
+    const uint64_t keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
+    const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
+    if (keep)
+        mhip::launch(ctx, mx4_kept_weights_kernel, dim3(static_cast<unsigned>(mhip::ceil_div(keys, 1024)), heads.y, heads.z),
+                     dim3(256), 0, a, weights, weights_out, stride);
+    else
+        mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(keys, 64 * kWeightWaves)), heads.y, heads.z),
+                     dim3(64 * kWeightWaves), 0, a, weights, weights_out, stride);
+    return mhip::check_launch("attention (4-bit, weights)");
 }
 
 }  // namespace
@@ -610,7 +801,6 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     a.causal = p->causal ? 1 : 0;
     a.window = p->window_size > 0 ? static_cast<int>(std::min<int64_t>(p->window_size, 1LL << 30)) : -1;
     a.vec = d % 4 == 0 && mhip::aligned16(out) && a.o_bs % 4 == 0;
-    a.row_tiles = static_cast<int>(mhip::ceil_div(rows, 16));
     const float scale = p->scale > 0.0f ? p->scale : 1.0f / std::sqrt(static_cast<float>(d));
     a.c = scale * kLog2e;
     if (p->bounded_key_count) {
@@ -620,14 +810,31 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
             (void)mhip::advance_ptr(ctx, MHIP_ADVANCE_KEY_COUNT, 0);
     }
     const uint64_t plan_rows = p->bounded_key_count ? p->kv_rows : p->kv_seq_len;
+    const bool few = a.rows <= kRowTile<true>;
     switch (mhip::mx4_blocks(d)) {
-        case 1: return launch_rows<1>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 2: return launch_rows<2>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 3: return launch_rows<3>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 4: return launch_rows<4>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 5: return launch_rows<5>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 6: return launch_rows<6>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        case 7: return launch_rows<7>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
-        default: return launch_rows<8>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 1:
+            return few ? launch_rows<1, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<1, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 2:
+            return few ? launch_rows<2, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<2, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 3:
+            return few ? launch_rows<3, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<3, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 4:
+            return few ? launch_rows<4, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<4, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 5:
+            return few ? launch_rows<5, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<5, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 6:
+            return few ? launch_rows<6, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<6, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        case 7:
+            return few ? launch_rows<7, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<7, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
+        default:
+            return few ? launch_rows<8, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
+                       : launch_rows<8, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);
     }
 }

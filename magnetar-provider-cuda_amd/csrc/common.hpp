@@ -25,6 +25,10 @@ struct mhip_ctx {
     // the last workgroup writes the answer into.
     uint64_t* select_state = nullptr;
     uint64_t* select_host = nullptr;
+    // Attention over 4-bit stores: a count of the key chunks done for each of
+    // up to mhip::kMx4Counters row tiles, zero between calls (each tile's last
+    // workgroup wraps its own).
+    uint32_t* mx4_arrived = nullptr;
     hipEvent_t timer_start = nullptr;
     hipEvent_t timer_stop = nullptr;
     uint32_t compute_units = 0;
@@ -75,6 +79,8 @@ struct mhip_ctx {
 };
 
 namespace mhip {
+
+constexpr uint64_t kMx4Counters = 4096;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));

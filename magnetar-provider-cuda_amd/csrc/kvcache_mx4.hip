@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(float* __restrict__ rows,
 // Eviction
 // ---------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectPer = 8;
 
 struct SelectArgs {
     const float* weights;  // [batch * heads][weight_stride]
@@ -191,74 +191,138 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// One workgroup per (sequence, head): the threshold weight by its bytes, the
-// highest first (a histogram of the candidates that match the bytes found so
-// far), then the rows above it and the first rows at it, in order.
+// One workgroup per (sequence, head). The threshold weight is found by its
+// bytes, the highest first: a histogram in LDS of the candidates that match
+// the bytes found so far, its running count from the top taken by every wave
+// for itself, so that a byte costs one barrier. Then, in one scan, the rows
+// above the threshold and the first ones at it, in order.
+//
+// A thread has kPer rows side by side. Up to kPer * 1024 rows their keys stay
+// in its registers over the five passes (CACHED); longer accounts are read
+// again, stretch by stretch. What it waits for is latency: a pass of 8192
+// weights is 4 loads a thread.
+template <bool CACHED>
 __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];             // the byte, and the rows still wanted within it
-    __shared__ uint32_t wave_sum[kSelectThreads / 64];
+    constexpr int kPer = kSelectPer;
+    constexpr uint32_t kStretch = kPer * kSelectThreads;
+    __shared__ uint32_t hist[4][256];
+    __shared__ uint32_t wave_above[kSelectThreads / 64], wave_equal[kSelectThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* w = a.weights + blockIdx.x * a.weight_stride;
     const uint32_t lo = a.first, hi = a.count - a.recent;  // the candidates
     uint32_t want = a.keep - a.first - a.recent;
+    const bool any = want > 0;
+    hist[tid >> 8][tid & 255] = 0;
+
+    uint32_t key[kPer];
+    float value[kPer];
+    auto load = [&](uint32_t base) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const uint32_t j = base + tid * kPer + e;
+            value[e] = j < a.count ? w[j] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) key[e] = weight_key(value[e]);
+    };
+    if (CACHED) load(0);
     uint32_t prefix = 0, mask = 0;
-    if (want > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (uint32_t j = lo + tid; j < hi; j += kSelectThreads) {
-                const uint32_t key = weight_key(w[j]);
-                if ((key & mask) == prefix) atomicAdd(&hist[key >> shift & 255], 1u);
+    __syncthreads();
+    if (any) {
+#pragma unroll
+        for (int pass = 0; pass < 4; ++pass) {
+            const int shift = 24 - 8 * pass;
+            for (uint32_t base = 0; base < a.count; base += kStretch) {
+                if (!CACHED) load(base);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const uint32_t j = base + tid * kPer + e;
+                    if (j >= lo && j < hi && (key[e] & mask) == prefix) atomicAdd(&hist[pass][key[e] >> shift & 255], 1u);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t left = want, v = 255;
-                while (v > 0 && hist[v] < left) left -= hist[v--];
-                found[0] = v;
-                found[1] = left;
+            // Lane l has the bytes 252 - 4 l to 255 - 4 l; the byte sought is
+            // the first from the top whose count reaches `want`.
+            uint32_t bin[4], mine = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                bin[x] = hist[pass][255 - 4 * lane - x];
+                mine += bin[x];
             }
-            __syncthreads();
-            prefix |= found[0] << shift;
+            uint32_t upto = mine;
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) {
+                const uint32_t v = static_cast<uint32_t>(__shfl_up(static_cast<int>(upto), off, 64));
+                if (lane >= off) upto += v;
+            }
+            const int at = __ffsll(static_cast<unsigned long long>(__ballot(upto >= want))) - 1;
+            uint32_t left = want - (upto - mine), byte = 255 - 4 * lane;
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+                if (byte == 255u - 4 * lane - x && bin[x] < left) {
+                    left -= bin[x];
+                    --byte;
+                }
+            want = static_cast<uint32_t>(__shfl(static_cast<int>(left), at, 64));
+            prefix |= static_cast<uint32_t>(__shfl(static_cast<int>(byte), at, 64)) << shift;
             mask |= 255u << shift;
-            want = found[1];
-            __syncthreads();
         }
     }
     // Kept: the forced rows and those above the threshold, and the first
     // `want` of those at it (none where no candidate is wanted).
-    const bool any = a.keep > a.first + a.recent;
-    uint32_t above_before = 0, equal_before = 0;
-    for (uint32_t base = 0; base < a.count; base += kSelectThreads) {
-        const uint32_t j = base + tid;
-        bool above = false, equal = false;
-        float value = 0.0f;
-        if (j < a.count) {
-            value = w[j];
-            const uint32_t key = weight_key(value);
+    uint32_t above_base = 0, equal_base = 0;
+    for (uint32_t base = 0; base < a.count; base += kStretch) {
+        if (!CACHED) load(base);
+        uint32_t above = 0, equal = 0;  // a bit a row
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const uint32_t j = base + tid * kPer + e;
             const bool forced = j < lo || j >= hi;
-            above = forced || (any && key > prefix);
-            equal = !forced && any && key == prefix;
+            if (j < a.count) {
+                if (forced || (any && key[e] > prefix)) above |= 1u << e;
+                if (!forced && any && key[e] == prefix) equal |= 1u << e;
+            }
         }
-        const uint64_t ba = __ballot(above), be = __ballot(equal);
-        const uint64_t below = (1ull << lane) - 1;
-        if (lane == 0) wave_sum[wave] = static_cast<uint32_t>(__popcll(ba)) | static_cast<uint32_t>(__popcll(be)) << 16;
+        uint32_t na = static_cast<uint32_t>(__popc(above)), ne = static_cast<uint32_t>(__popc(equal));
+        const uint32_t own_a = na, own_e = ne;
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) {
+            const uint32_t va = static_cast<uint32_t>(__shfl_up(static_cast<int>(na), off, 64));
+            const uint32_t ve = static_cast<uint32_t>(__shfl_up(static_cast<int>(ne), off, 64));
+            if (lane >= off) {
+                na += va;
+                ne += ve;
+            }
+        }
+        if (lane == 63) {
+            wave_above[wave] = na;
+            wave_equal[wave] = ne;
+        }
         __syncthreads();  // also: every read of this stretch of weights is done
-        uint32_t before = 0, total = 0;
+        na += above_base - own_a;
+        ne += equal_base - own_e;
+#pragma unroll
         for (int i = 0; i < kSelectThreads / 64; ++i) {
-            if (i < wave) before += wave_sum[i];
-            total += wave_sum[i];
+            const uint32_t va = wave_above[i], ve = wave_equal[i];
+            if (i < wave) {
+                na += va;
+                ne += ve;
+            }
+            above_base += va;
+            equal_base += ve;
         }
-        const uint32_t na = above_before + (before & 0xFFFF) + static_cast<uint32_t>(__popcll(ba & below));
-        const uint32_t ne = equal_before + (before >> 16) + static_cast<uint32_t>(__popcll(be & below));
-        if (above || (equal && ne < want)) {
-            const uint32_t to = na + min(ne, want);
-            a.indices[static_cast<uint64_t>(blockIdx.x) * a.keep + to] = j;
-            a.weights_out[blockIdx.x * a.out_stride + to] = value;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const bool is_above = above >> e & 1, is_equal = equal >> e & 1;
+            if (is_above || (is_equal && ne < want)) {
+                const uint32_t to = na + min(ne, want);
+                a.indices[static_cast<uint64_t>(blockIdx.x) * a.keep + to] = base + tid * kPer + e;
+                a.weights_out[blockIdx.x * a.out_stride + to] = value[e];
+            }
+            na += is_above;
+            ne += is_equal;
         }
-        above_before += total & 0xFFFF;
-        equal_before += total >> 16;
-        __syncthreads();
+        if (!CACHED) __syncthreads();
     }
     // The rows that come next start at nothing.
     for (uint32_t j = a.keep + tid; j < a.out_rows; j += kSelectThreads) a.weights_out[blockIdx.x * a.out_stride + j] = 0.0f;
@@ -472,6 +536,7 @@ extern "C" mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, con
         return mhip::fail(MHIP_LAYOUT_UNSUPPORTED,
                           "kv-evict: the output stores overlap the stores (in place: the same stores and shape)");
     const uint64_t rows = batch * heads;
+    if (rows >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-evict: too many heads");
     const uint64_t w_bytes = (rows - 1) * w_stride * 4 + p->key_count * 4;
     const uint64_t o_bytes = (rows - 1) * o_stride * 4 + out_shape->capacity * 4;
     if (!(weights_out == weights && w_stride == o_stride) && overlap(weights, w_bytes, weights_out, o_bytes))
@@ -500,7 +565,10 @@ extern "C" mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, con
     sel.first = static_cast<uint32_t>(p->first);
     sel.recent = static_cast<uint32_t>(p->recent);
     sel.out_rows = static_cast<uint32_t>(out_shape->capacity);
-    mhip::launch(ctx, mx4_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, sel);
+    if (p->key_count <= kSelectThreads * kSelectPer)
+        mhip::launch(ctx, mx4_select_kernel<true>, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, sel);
+    else
+        mhip::launch(ctx, mx4_select_kernel<false>, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, sel);
     st = mhip::check_launch("kv-evict (select)");
     if (st != MHIP_OK || p->keep == 0) return st;
 

@@ -235,6 +235,8 @@ mhip_status mhip_ctx_create(int ordinal, mhip_ctx** out) {
         (err = hipMemset(ctx->flags, 0, 256)) != hipSuccess ||
         (err = hipMalloc(reinterpret_cast<void**>(&ctx->select_state), 256)) != hipSuccess ||
         (err = hipMemset(ctx->select_state, 0, 256)) != hipSuccess ||
+        (err = hipMalloc(reinterpret_cast<void**>(&ctx->mx4_arrived), mhip::kMx4Counters * 4)) != hipSuccess ||
+        (err = hipMemset(ctx->mx4_arrived, 0, mhip::kMx4Counters * 4)) != hipSuccess ||
         (err = hipHostMalloc(reinterpret_cast<void**>(&ctx->select_host), 256,
                              hipHostMallocCoherent)) != hipSuccess ||
         // The context's stream does not wait for the null stream's memsets.
@@ -259,6 +261,7 @@ mhip_status mhip_ctx_destroy(mhip_ctx* ctx) {
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->flags) (void)hipFree(ctx->flags);
     if (ctx->select_state) (void)hipFree(ctx->select_state);
+    if (ctx->mx4_arrived) (void)hipFree(ctx->mx4_arrived);
     if (ctx->select_host) (void)hipHostFree(ctx->select_host);
     for (auto& table : ctx->rope_tables) (void)hipFree(table.device);
     if (ctx->workspace) (void)hipFree(ctx->workspace);
