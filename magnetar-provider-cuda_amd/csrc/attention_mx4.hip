@@ -60,8 +60,13 @@ struct Mx4Attn {
     int heads, kv_heads, group, d, groups;
     int causal, window;           // window -1: none
     int vec;                      // rows of q and out are whole float4s
-    int row_tiles, chunks;
+    int vec_q;                    // rows of q are whole float4s
+    int row_tiles, heavy_ranks, chunks, chunk_tiles, batch;
     float c;                      // scale * log2(e)
+    char* tiles;                  // [batch][kv head][tile] PromptCfg::kBytes
+    uint64_t tiles_ld;
+    char* planes;                 // [batch][kv head][32 rows] SumCfg::kBytes (weights asked for)
+    uint64_t planes_ld;
     float* part_o;                // [batch][kv head][row tile][chunk][row][DP]
     float* part_ml;               // [batch][kv head][row tile][chunk][row][2]
     uint32_t* arrived;            // [batch][kv head][row tile]: chunks done, 0 between calls
@@ -75,6 +80,9 @@ struct Mx4Attn {
 struct Keys {
     int lo, hi;
 };
+__device__ __forceinline__ bool outside(const Keys& k, int key) {  // one comparison
+    return static_cast<uint32_t>(key - k.lo) >= static_cast<uint32_t>(k.hi - k.lo);
+}
 __device__ __forceinline__ Keys row_keys(const Mx4Attn& a, int kv, int row) {
     const int at = kv - a.seq + row / a.group;
     Keys k;
@@ -256,6 +264,15 @@ __device__ __forceinline__ void outputs(const Strip<NB>& v, const float (&p)[4][
     }
 }
 
+__device__ __forceinline__ uint32_t bytes_255(uint32_t x) {  // bit 7 of each byte that is 255
+    return ((x & 0x7F7F7F7Fu) + 0x01010101u) & x & 0x80808080u;
+}
+// ... a bit each, byte i's bit i.
+__device__ __forceinline__ uint32_t byte_bits(uint32_t ff) {
+    return (ff >> 7 & 1u) | (ff >> 14 & 2u) | (ff >> 21 & 4u) | (ff >> 28 & 8u);
+}
+__device__ __forceinline__ uint32_t whole_bytes(uint32_t ff) { return ff | (ff - (ff >> 7)); }
+
 // In a strip at a mask's edge a value that is no number may belong to a key
 // that some rows admit and others do not, and to the product 0 times it is no
 // number for all of them. Its block is taken out of the strip (scale byte 0:
@@ -266,19 +283,18 @@ __device__ __forceinline__ void edge_values(Strip<NB>& v, int base, int g, const
     uint32_t flags[NB];  // bit 4 r + i: the block of key 16 g + 4 r + i is no number
     uint32_t any = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        flags[b] = 0;
+    for (int b = 0; b < NB; ++b) flags[b] = 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
+        const int live = min(max(hi - (base + 16 * g + 4 * r), 0), 4);  // keys of the unit before `hi`
+        const uint32_t keep = static_cast<uint32_t>((1ull << (8 * live)) - 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t byte = 255u << (8 * i);
-                const bool nan = (v.scale[r].w[b] & byte) == byte;
-                const bool past = base + 16 * g + 4 * r + i >= hi;
-                if (nan || past) v.scale[r].w[b] &= ~byte;
-                if (nan && !past) flags[b] |= 1u << (4 * r + i);
-            }
-        any |= flags[b];
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t scale = v.scale[r].w[b] & keep, ff = bytes_255(scale);
+            v.scale[r].w[b] = scale & ~whole_bytes(ff);
+            flags[b] |= byte_bits(ff) << (4 * r);
+            any |= ff;
+        }
     }
     if (__ballot(any != 0) == 0) return;
 #pragma unroll
@@ -410,14 +426,14 @@ __global__ __launch_bounds__(64 * kRowWaves<NB>) void mx4_rows_kernel(Mx4Attn a)
             for (int r = 0; r < 4; ++r)
                 *reinterpret_cast<f32x4*>(to + 4 * r) = f32x4{st[0][r], st[1][r], st[2][r], st[3][r]};
         }
-        const bool edge = base < tail.lo || base + 64 > head.hi;
-        if (edge) {
+        if (base < tail.lo || base + 64 > head.hi) {
+            asm volatile("");  // a branch
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int key = base + 16 * g + 4 * r + i;
-                    if (key < mine.lo || key >= mine.hi) st[i][r] = -INFINITY;
+                    if (outside(mine, key)) st[i][r] = -INFINITY;
                 }
             edge_values<NB>(v, base, g, mine, tail.hi, o);
         }
@@ -596,6 +612,609 @@ __global__ __launch_bounds__(64 * kRowWaves<NB>) void mx4_rows_kernel(Mx4Attn a)
     }
 }
 
+// ---------------------------------------------------------------------------
+// Prompts
+// ---------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+
+__device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+
+// The scores of a prompt come from the block-scaled matrix instructions, which
+// take K's codes and scale bytes as they are held, and Q as planes of six bits
+// (E2M3: with magnitudes below 2 under its scale, multiples of 1/8). A plane is
+// the nearest to what the planes before it leave, at most 1/16 of their unit,
+// so each adds five bits: six planes hold a block of 32 values of Q to within
+// 2^-30 of its largest one, and add up in f32, the smallest first. Six such
+// products take the time of one and a half in bf16, and K needs no conversion.
+// (Five planes: 6.7e-8 of the scores' norm off, an f32 chain of multiply-adds
+// 1.4e-7, six 3.0e-8; with one value of a block 1000 times the others and keys
+// that are zero there, 2.6e-5 and 7.9e-7.)
+constexpr int kQPlanes = 6;
+template <int NB, bool MADE>
+struct QPlanes {
+    static constexpr int kSteps = (NB + 1) / 2;  // of two blocks, one a half of the wave
+    // Above two blocks, with the units that a thread carries, the registers do not
+    // hold all: planes 3 to 5 stay in LDS.
+    static constexpr bool kLow = NB > 2 && !MADE;
+    u32x6 f[kSteps][kQPlanes];
+    uint32_t scale[kSteps][2];  // scale bytes of planes 0-3 and 4-5
+};
+
+// A plane of one lane in LDS, 16 and 8 bytes side by side over the lanes
+// (`p`: the plane's place, at the lane's 16 bytes).
+constexpr int kPlaneBytes = 64 * 24;
+__device__ __forceinline__ void store_plane(char* p, const u32x6& f) {
+    const uint4 x = {f[0], f[1], f[2], f[3]};
+    const uint2 y = {f[4], f[5]};
+    *reinterpret_cast<uint4*>(p) = x;
+    *reinterpret_cast<uint2*>(p + 1024 - 8 * (threadIdx.x & 63)) = y;
+}
+__device__ __forceinline__ u32x6 load_plane(const char* p) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const uint2 y = *reinterpret_cast<const uint2*>(p + 1024 - 8 * (threadIdx.x & 63));
+    return u32x6{x.x, x.y, x.z, x.w, y.x, y.y};
+}
+
+// Lane (row, h), step s: block 2 s + h of the row (32 NB values in LDS, zeros
+// past d), its values 2 i and 2 i + 1 the block's columns i and 16 + i, as the
+// codes of K lie.
+template <int NB, bool MADE>
+__device__ __forceinline__ void make_q_planes(const float* qrow, int h, QPlanes<NB, MADE>& q) {
+#pragma unroll
+    for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s) {
+        const int p = 2 * s + h;
+        f32x16 lo, hi;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(qrow + 32 * min(p, NB - 1) + 4 * i);
+            const f32x4 y = *reinterpret_cast<const f32x4*>(qrow + 32 * min(p, NB - 1) + 16 + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                lo[4 * i + e] = p < NB ? x[e] : 0.0f;
+                hi[4 * i + e] = p < NB ? y[e] : 0.0f;
+                top = max(top, max(__float_as_uint(lo[4 * i + e]) & 0x7FFFFFFFu, __float_as_uint(hi[4 * i + e]) & 0x7FFFFFFFu));
+            }
+        }
+        // Magnitudes below 2 under 2^(e - 127), the last plane's byte above 0.
+        const uint32_t e = max(top >> 23, 5u * kQPlanes);
+        const bool nan = top >= 0x7F800000u;
+        uint32_t bytes[2] = {0, 0};
+#pragma unroll
+        for (int n = 0; n < kQPlanes; ++n) {
+            const uint32_t en = e - 5 * n;
+            const float scale = __uint_as_float(en << 23);
+            q.f[s][n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(lo, hi, scale);
+            bytes[n / 4] |= (nan ? 255u : en) << (8 * (n % 4));
+            if (n + 1 < kQPlanes) {
+                const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q.f[s][n], scale);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    lo[i] -= held[2 * i];
+                    hi[i] -= held[2 * i + 1];
+                }
+            }
+        }
+        q.scale[s][0] = bytes[0];
+        q.scale[s][1] = bytes[1];
+    }
+}
+
+// Four columns of a row of q, zeros past d.
+__device__ __forceinline__ f32x4 load_q4(const Mx4Attn& a, const float* qrow, int col) {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.vec_q) {
+        if (col < a.d) x = *reinterpret_cast<const f32x4*>(qrow + col);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < a.d) x[e] = qrow[col + e];
+    }
+    return x;
+}
+
+// c += K (32 keys, block 2 s + h a lane half) by plane N of Q.
+template <int OPK, int OPQ>
+__device__ __forceinline__ f32x16 scaled_product(const Frag& k, uint32_t kscale, const u32x6& q, uint32_t qscale, f32x16 c) {
+    const i32x8 x = {static_cast<int>(k.u[0]), static_cast<int>(k.u[1]), static_cast<int>(k.u[2]), static_cast<int>(k.u[3]), 0, 0, 0, 0};
+    const i32x8 y = {static_cast<int>(q[0]), static_cast<int>(q[1]), static_cast<int>(q[2]),
+                     static_cast<int>(q[3]), static_cast<int>(q[4]), static_cast<int>(q[5]), 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, OPK, static_cast<int>(kscale), OPQ, static_cast<int>(qscale));
+}
+// st[0] and st[1] (two chains) += 32 keys each by all planes of Q, the smallest
+// first. `low`: planes 3 to 5 of the step, from LDS.
+template <int OPK, int NB, bool MADE>
+__device__ __forceinline__ void score_step(const Frag& k0, const Frag& k1, uint32_t s0, uint32_t s1, const QPlanes<NB, MADE>& q, int s,
+                                           const char* low, f32x16 (&st)[2]) {
+    u32x6 f[3];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        if constexpr (QPlanes<NB, MADE>::kLow)
+            f[n] = load_plane(low + (3 * s + n) * kPlaneBytes);
+        else
+            f[n] = q.f[s][3 + n];
+    }
+    st[0] = scaled_product<OPK, 1>(k0, s0, f[2], q.scale[s][1], st[0]);
+    st[1] = scaled_product<OPK, 1>(k1, s1, f[2], q.scale[s][1], st[1]);
+    st[0] = scaled_product<OPK, 0>(k0, s0, f[1], q.scale[s][1], st[0]);
+    st[1] = scaled_product<OPK, 0>(k1, s1, f[1], q.scale[s][1], st[1]);
+    st[0] = scaled_product<OPK, 3>(k0, s0, f[0], q.scale[s][0], st[0]);
+    st[1] = scaled_product<OPK, 3>(k1, s1, f[0], q.scale[s][0], st[1]);
+    st[0] = scaled_product<OPK, 2>(k0, s0, q.f[s][2], q.scale[s][0], st[0]);
+    st[1] = scaled_product<OPK, 2>(k1, s1, q.f[s][2], q.scale[s][0], st[1]);
+    st[0] = scaled_product<OPK, 1>(k0, s0, q.f[s][1], q.scale[s][0], st[0]);
+    st[1] = scaled_product<OPK, 1>(k1, s1, q.f[s][1], q.scale[s][0], st[1]);
+    st[0] = scaled_product<OPK, 0>(k0, s0, q.f[s][0], q.scale[s][0], st[0]);
+    st[1] = scaled_product<OPK, 0>(k1, s1, q.f[s][0], q.scale[s][0], st[1]);
+}
+
+#ifndef SB
+#define SB 4
+#endif
+#ifndef MC
+#define MC 8
+#endif
+constexpr uint64_t kSplitBelow = SB, kMinChunk = MC;
+#ifndef MF
+#define MF 4
+#endif
+constexpr int kMadeFrom = MF;
+constexpr float kLag = 8.0f;
+constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
+
+// Four waves of 32 rows share tiles of 64 keys in LDS, each thread carrying one
+// unit of K and one of V there from the stores:
+//
+//   K as codes, [half of 32 keys][block][key] 16 bytes (the blocks 16 bytes
+//     apart in the banks). A unit has one byte of each of 4 NB (key, block)
+//     pairs; four lanes transpose theirs to write four bytes of a pair at once.
+//     Behind them a key's scale bytes, a dword a key.
+//   V as bf16 operands of 32x32x16 products, [half][step of 16 keys][block][lane]
+//     16 bytes, lane (m, h) the keys 4 h to 4 h + 3 and 8 + 4 h to 11 + 4 h of
+//     column m of the block: the keys whose weights that half of the wave has
+//     after the scores.
+template <int NB, bool MADE = true>
+struct PromptCfg {
+    static constexpr int kBlock = 32 * 16 + 16;
+    static constexpr int kKHalf = NB * kBlock + 128;  // codes, scales
+    static constexpr int kVHalf = 2 * NB * 1024;
+    static constexpr int kNan = 2 * (kKHalf + kVHalf);  // behind the tile: its NaN bits, [block][half]
+    static constexpr int kBytes = (kNan + 8 * NB + 1023) / 1024 * 1024;
+    // A wave's rows of q or of the output pass through LDS, 16 bytes apart in
+    // the banks, so that memory is read and written along the rows.
+    static constexpr int kRow = 32 * NB + 4;  // floats
+    static constexpr int kLowBytes = QPlanes<NB, MADE>::kLow ? 3 * QPlanes<NB, MADE>::kSteps * kPlaneBytes : 0;  // a wave
+    static constexpr int kLoop = 2 * kBytes + kPromptWaves * kLowBytes, kRows = kPromptWaves * 32 * kRow * 4;
+    static constexpr int kLds = kLoop > kRows ? kLoop : kRows;
+};
+
+// The planes of Q of 32 rows as the weights' kernel takes them: [step][plane]
+// kPlaneBytes, then the scale bytes [step][lane] 8 bytes.
+template <int NB>
+struct SumCfg {
+    static constexpr int kSteps = (NB + 1) / 2;
+    static constexpr int kBytes = (kSteps * (kQPlanes * kPlaneBytes + 512) + 1023) / 1024 * 1024;
+};
+
+// What a thread carries from memory to LDS: a unit of each store with its scales.
+template <int NB>
+struct Carry {
+    Mx4Unit<NB> k, ks, v, vs;
+};
+
+template <int NB>
+__device__ __forceinline__ void load_carry(const Mx4Attn& a, int b, int kvh, int t, int kg, int n, Carry<NB>& c) {
+    const uint8_t* ks = a.k + b * a.k_bs;
+    const uint8_t* vs = a.v + b * a.v_bs;
+    const uint64_t g = static_cast<uint64_t>(kvh) * a.groups + min(t * 16 + kg, (a.kv - 1) / 4);
+    c.k = mhip::mx4_load<NB>(reinterpret_cast<const uint32_t*>(ks) + (g * 16 + n) * NB);
+    c.ks = mhip::mx4_load<NB>(reinterpret_cast<const uint32_t*>(ks + a.code_bytes) + g * NB);
+    c.v = mhip::mx4_load<NB>(reinterpret_cast<const uint32_t*>(vs) + (g * 16 + n) * NB);
+    c.vs = mhip::mx4_load<NB>(reinterpret_cast<const uint32_t*>(vs + a.code_bytes) + g * NB);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xF, 0xF, true));
+}
+
+// K of a tile: group kg of four keys, unit n.
+template <int NB>
+__device__ __forceinline__ void store_keys(const Carry<NB>& c, char* lds, int kg, int n) {
+    using Cfg = PromptCfg<NB>;
+    const int half = kg >> 3, j = kg & 7, lane4 = n & 3;
+    char* kd = lds + half * Cfg::kKHalf;
+    const uint32_t sel1 = lane4 & 1 ? 0x03070105u : 0x06020400u, sel2 = lane4 & 2 ? 0x03020706u : 0x05040100u;
+#pragma unroll
+    for (int w = 0; w < NB; ++w) {
+        const uint32_t x = __builtin_amdgcn_perm(quad<0xB1>(c.k.w[w]), c.k.w[w], sel1);  // lane ^ 1
+        const uint32_t y = __builtin_amdgcn_perm(quad<0x4E>(x), x, sel2);                // lane ^ 2
+        const int at = 4 * w + lane4, i = at / NB, p = at % NB;
+        *reinterpret_cast<uint32_t*>(kd + p * Cfg::kBlock + (4 * j + i) * 16 + (n & ~3)) = y;
+    }
+    uint32_t s = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) s |= (p < NB ? c.ks.w[p < NB ? p : 0] >> (8 * lane4) & 255u : 127u) << (8 * p);
+    if (n < 4) *reinterpret_cast<uint32_t*>(kd + NB * Cfg::kBlock + (4 * j + n) * 4) = s;
+}
+
+// `nan`: a tile's keys of each block whose value is no number, a bit a key.
+// Those values go to LDS as zeros; the rows that admit the key get their NaN
+// from the bits (a weight of 0 times NaN would reach the others too).
+template <int NB>
+__device__ __forceinline__ void take_nan(Carry<NB>& c, uint32_t (*nan)[2], int kg, int n) {
+    const int half = kg >> 3, j = kg & 7;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int p = 0; p < NB; ++p) bad |= bytes_255(c.vs.w[p]);
+    if (bad) {
+#pragma unroll
+        for (int p = 0; p < NB; ++p) {
+            const uint32_t ff = bytes_255(c.vs.w[p]);
+            c.vs.w[p] &= ~whole_bytes(ff);
+            if (n == 0 && ff) atomicOr(&nan[p][half], byte_bits(ff) << (4 * j));
+        }
+    }
+}
+
+// V of a tile.
+template <int NB>
+__device__ __forceinline__ void store_values(const Carry<NB>& c, char* lds, int kg, int n) {
+    using Cfg = PromptCfg<NB>;
+    const int half = kg >> 3, j = kg & 7;
+    char* vd = lds + 2 * Cfg::kKHalf + half * Cfg::kVHalf + ((j / 4) * NB * 64 + (j & 1) * 32 + n) * 16 + (j & 2) * 4;
+#pragma unroll
+    for (int p = 0; p < NB; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = i * NB + p;
+            w[i] = bits(mhip::mx4_bf16(c.v.w[at / 4], mhip::mx4_scale(c.vs.w[p], i), at % 4));
+        }
+        const uint2 lo = {__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+        const uint2 hi = {__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+        *reinterpret_cast<uint2*>(vd + p * 1024) = lo;
+        *reinterpret_cast<uint2*>(vd + p * 1024 + 256) = hi;
+    }
+}
+
+__device__ __forceinline__ Frag lds_frag(const char* p) {
+    Frag f;
+    __builtin_memcpy(&f, __builtin_assume_aligned(p, 16), 16);
+    return f;
+}
+
+// S^T of a tile's 64 keys by the wave's 32 rows: st[kk][r] is key 32 kk + 8 (r /
+// 4) + 4 h + r % 4 of row lane % 32.
+template <int NB, bool MADE>
+__device__ __forceinline__ void tile_scores(const char* kt, const QPlanes<NB, MADE>& q, const char* low, int m, int h, f32x16 (&st)[2]) {
+    using Cfg = PromptCfg<NB>;
+    const char* k0 = kt;
+    const char* k1 = kt + Cfg::kKHalf;
+    const uint32_t scale0 = *reinterpret_cast<const uint32_t*>(k0 + NB * Cfg::kBlock + m * 4) >> (8 * h);
+    const uint32_t scale1 = *reinterpret_cast<const uint32_t*>(k1 + NB * Cfg::kBlock + m * 4) >> (8 * h);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[0][e] = st[1][e] = 0.0f;
+    constexpr int kSteps = QPlanes<NB, MADE>::kSteps;
+    Frag k[kSteps][2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int at = min(2 * i + h, NB - 1) * Cfg::kBlock + m * 16;
+        k[i][0] = lds_frag(k0 + at);
+        k[i][1] = lds_frag(k1 + at);
+    }
+    score_step<0>(k[0][0], k[0][1], scale0, scale1, q, 0, low, st);
+    if constexpr (kSteps > 1) score_step<2>(k[1][0], k[1][1], scale0, scale1, q, 1, low, st);
+}
+
+// 16 bytes a lane from memory to 1024 bytes of LDS, whose address is the
+// wave's. As an instruction of its own: the compiler has every read of LDS wait
+// for the builtin's, here the tile in use for the one after it (95 us for 80
+// over a prompt of 2048). Its caller waits for vmcnt before the barrier that
+// gives the tile to the other waves.
+__device__ __forceinline__ void copy_to_lds(const char* from, char* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+}
+
+// The words of a tile's NaN bits together.
+__device__ __forceinline__ uint32_t any_nan(const uint32_t* flags, int words) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < words; ++i) any |= flags[i];
+    return any;
+}
+
+// A prompt's place in the grid: the heaviest (latest) row tiles first over all
+// heads, then the chunks of a row tile, `chunk_tiles` tiles each. Of a grid of
+// two workgroups a CU the second halves go up from the lightest, so that a CU
+// gets one with the other.
+struct PromptPlace {
+    int b, kvh, tile, chunk;
+    int row0, row_last;
+    int t0, t1;     // the chunk's tiles
+    int chunks;     // of this row tile
+};
+__device__ __forceinline__ PromptPlace prompt_place(const Mx4Attn& a, int block) {
+    PromptPlace w;
+    const int pairs = a.kv_heads * a.batch;
+    const int unit = block / pairs, pair = block - unit * pairs;
+    const int rank = a.chunks > 1 ? unit / a.chunks : unit;
+    w.chunk = a.chunks > 1 ? unit - rank * a.chunks : 0;
+    w.tile = rank < a.heavy_ranks ? a.row_tiles - 1 - rank : rank - a.heavy_ranks;
+    w.b = pair / a.kv_heads;
+    w.kvh = pair - w.b * a.kv_heads;
+    w.row0 = w.tile * kPromptRows;
+    w.row_last = min(w.row0 + kPromptRows, a.rows) - 1;
+    const int begin = row_keys(a, a.kv, w.row0).lo / 64, end = (row_keys(a, a.kv, w.row_last).hi + 63) / 64;
+    w.chunks = a.chunks > 1 ? (end - begin + a.chunk_tiles - 1) / a.chunk_tiles : 1;
+    w.t0 = begin + w.chunk * a.chunk_tiles;
+    w.t1 = a.chunks > 1 ? min(w.t0 + a.chunk_tiles, end) : end;
+    return w;
+}
+
+// The tiles of a KV head as the workgroups' LDS takes them, made once where
+// several workgroups read each: [sequence][KV head][tile] kBytes.
+template <int NB>
+__global__ __launch_bounds__(256) void mx4_tiles_kernel(Mx4Attn a) {
+    using Cfg = PromptCfg<NB>;
+    __shared__ __attribute__((aligned(16))) char lds[Cfg::kBytes];
+    const int tid = threadIdx.x, kg = tid >> 4, n = tid & 15;
+    const int t = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    uint32_t(*nan)[2] = reinterpret_cast<uint32_t(*)[2]>(lds + Cfg::kNan);
+    if (tid < 2 * NB) (&nan[0][0])[tid] = 0;
+    Carry<NB> c;
+    load_carry<NB>(a, b, kvh, t, kg, n, c);
+    __syncthreads();
+    take_nan<NB>(c, nan, kg, n);
+    store_keys<NB>(c, lds, kg, n);
+    store_values<NB>(c, lds, kg, n);
+    __syncthreads();
+    uint4* to = reinterpret_cast<uint4*>(a.tiles + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.tiles_ld + t) * Cfg::kBytes);
+    for (int i = tid; i < (Cfg::kNan + 8 * NB + 15) / 16; i += 256) to[i] = reinterpret_cast<const uint4*>(lds)[i];
+}
+
+template <int NB, bool MADE>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Attn a) {
+    using Cfg = PromptCfg<NB, MADE>;
+    constexpr int DP = 32 * NB;
+    __shared__ __attribute__((aligned(16))) char lds[Cfg::kLds];
+    __shared__ uint32_t nan[3][NB][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = lane & 31, h = lane >> 5, kg = tid >> 4, n = tid & 15;
+    const PromptPlace at = prompt_place(a, blockIdx.x);
+    if (at.chunk >= at.chunks) return;
+    const int b = at.b, kvh = at.kvh, t0 = at.t0, t1 = at.t1;
+
+    const int wrow0 = min(at.row0 + wave * 32, a.rows - 1), wrow_last = min(wrow0 + 31, a.rows - 1);
+    const int row = min(at.row0 + wave * 32 + q, a.rows - 1);
+    const bool wave_live = at.row0 + wave * 32 < a.rows;
+    const Keys mine = row_keys(a, a.kv, row);
+    const Keys whead = row_keys(a, a.kv, wrow0), wtail = row_keys(a, a.kv, wrow_last);
+
+    // MADE: the tiles come as they are, straight to LDS; else from the stores.
+    Carry<NB> carry;
+    const char* made = MADE ? a.tiles + (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.tiles_ld * Cfg::kBytes : nullptr;
+    auto fetch = [&](int t, char* to) {
+        const char* from = made + static_cast<uint64_t>(t) * Cfg::kBytes;
+#pragma unroll
+        for (int i = 0; i < (Cfg::kBytes / 1024 + kPromptWaves - 1) / kPromptWaves; ++i) {
+            const int part = i * kPromptWaves + wave;
+            if (part < Cfg::kBytes / 1024)
+                copy_to_lds(from + part * 1024 + lane * 16, to + part * 1024);
+        }
+    };
+    if (!MADE) load_carry<NB>(a, b, kvh, t0, kg, n, carry);
+    float* wrows = reinterpret_cast<float*>(lds) + wave * 32 * Cfg::kRow;
+    for (int u = lane; u < 8 * DP; u += 64) {
+        const int r = u / (DP / 4), col = u % (DP / 4) * 4;
+        const int from = min(at.row0 + wave * 32 + r, a.rows - 1);
+        *reinterpret_cast<f32x4*>(wrows + r * Cfg::kRow + col) = load_q4(a, a.q + b * a.q_bs + row_at(a, kvh, from), col);
+    }
+    if (tid < 6 * NB) (&nan[0][0][0])[tid] = 0;
+    __syncthreads();
+    QPlanes<NB, MADE> qp;
+    make_q_planes<NB, MADE>(wrows + q * Cfg::kRow, h, qp);
+    __syncthreads();
+    char* low = lds + 2 * Cfg::kBytes + wave * Cfg::kLowBytes + lane * 16;
+    if (a.planes && at.chunk == 0 && wave_live) {
+        char* keep = a.planes + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.planes_ld + at.tile * kPromptWaves + wave) * SumCfg<NB>::kBytes;
+#pragma unroll
+        for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s) {
+#pragma unroll
+            for (int n = 0; n < kQPlanes; ++n) store_plane(keep + (s * kQPlanes + n) * kPlaneBytes + lane * 16, qp.f[s][n]);
+            *reinterpret_cast<uint2*>(keep + QPlanes<NB, MADE>::kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8) = uint2{qp.scale[s][0], qp.scale[s][1]};
+        }
+    }
+    if constexpr (QPlanes<NB, MADE>::kLow)
+#pragma unroll
+        for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s)
+#pragma unroll
+            for (int n = 0; n < 3; ++n) store_plane(low + (3 * s + n) * kPlaneBytes, qp.f[s][3 + n]);
+    if constexpr (MADE) {
+        fetch(t0, lds);
+    } else {
+        take_nan<NB>(carry, nan[0], kg, n);
+        store_keys<NB>(carry, lds, kg, n);
+        store_values<NB>(carry, lds, kg, n);
+        load_carry<NB>(a, b, kvh, t0 + 1, kg, n, carry);
+    }
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    int slot = 0;  // (t - t0) % 3
+    for (int t = t0; t < t1; ++t) {
+        const int base = 64 * t, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
+        if (MADE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile is in LDS
+        __syncthreads();
+        if (!MADE && tid < 2 * NB) (&nan[after][0][0])[tid] = 0;
+        const char* kt = lds + ((t - t0) & 1) * Cfg::kBytes;
+        const char* vt = kt + 2 * Cfg::kKHalf;
+        char* to = lds + ((t + 1 - t0) & 1) * Cfg::kBytes;
+        if constexpr (MADE) {
+            if (t + 1 < t1) fetch(t + 1, to);
+        } else {
+            take_nan<NB>(carry, nan[next], kg, n);
+        }
+        if (!(wave_live && base < wtail.hi && base + 64 > whead.lo)) {
+            if constexpr (!MADE) {
+                store_keys<NB>(carry, to, kg, n);
+                store_values<NB>(carry, to, kg, n);
+                load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
+            }
+        } else {
+            f32x16 st[2];
+            const uint32_t no_number = any_nan(MADE ? reinterpret_cast<const uint32_t*>(kt + Cfg::kNan) : &nan[slot][0][0], 2 * NB);
+            tile_scores<NB, MADE>(kt, qp, low, q, h, st);
+            if constexpr (!MADE) {
+                store_keys<NB>(carry, to, kg, n);
+                store_values<NB>(carry, to, kg, n);
+                load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
+            }
+            if (base < wtail.lo || base + 64 > whead.hi) {
+                asm volatile("");  // a branch: 96 instructions that few tiles need
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = base + 32 * kk + 8 * (e / 4) + 4 * h + e % 4;
+                        if (outside(mine, key)) st[kk][e] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, st[kk][e]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // The maximum moves only when a score passes it by 2^8: weights of up
+            // to 2^8 are as exact, and few tiles then rescale the sums.
+            top *= a.c;
+            if (__ballot(top > m + kLag) != 0) {
+                const float m_new = fmaxf(m, top);
+                const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+                m = m_new;
+                l *= alpha;
+#pragma unroll
+                for (int c = 0; c < NB; ++c)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[c][e] *= alpha;
+            }
+            const float m_use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kk][8 * u + e], a.c, -m_use));
+                        l += p[e];
+                    }
+                    Frag w[3];
+                    split8(p, w);
+#pragma unroll
+                    for (int c = 0; c < NB; ++c) {
+                        const Frag f = lds_frag(vt + kk * Cfg::kVHalf + ((u * NB + c) * 64 + lane) * 16);
+                        o[c] = mfma32(f, w[2], o[c]);
+                        o[c] = mfma32(f, w[1], o[c]);
+                        o[c] = mfma32(f, w[0], o[c]);
+                    }
+                }
+            if (__builtin_amdgcn_readfirstlane(no_number) != 0) {
+                asm volatile("");  // a branch
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    const uint32_t* flags = MADE ? reinterpret_cast<const uint32_t*>(kt + Cfg::kNan) + 2 * c : nan[slot][c];
+                    const uint64_t bad = static_cast<uint64_t>(flags[1]) << 32 | flags[0];
+                    const int lo = min(max(mine.lo - base, 0), 64), hi = min(max(mine.hi - base, 0), 64);
+                    const uint64_t mask = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
+                    if (bad & mask)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[c][e] = NAN;
+                }
+            }
+        }
+        slot = next;
+    }
+    l += __shfl_xor(l, 32, 64);
+    // The outputs of several chunks as they are, else divided, along the rows.
+    const float inv = 1.0f / l, f = at.chunks > 1 ? 1.0f : inv;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<f32x4*>(wrows + q * Cfg::kRow + 32 * c + 8 * e + 4 * h) =
+                f32x4{o[c][4 * e] * f, o[c][4 * e + 1] * f, o[c][4 * e + 2] * f, o[c][4 * e + 3] * f};
+    __syncthreads();
+    const uint64_t pair = static_cast<uint64_t>(b) * a.kv_heads + kvh;
+    const uint64_t rec = ((pair * a.row_tiles + at.tile) * a.chunks + at.chunk) * kPromptRows + wave * 32;
+    const int wlive = min(a.rows - at.row0 - wave * 32, 32);
+    for (int u = lane; u < wlive * (DP / 4); u += 64) {
+        const int r = u / (DP / 4), col = u % (DP / 4) * 4;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(wrows + r * Cfg::kRow + col);
+        if (at.chunks > 1)
+            *reinterpret_cast<f32x4*>(a.part_o + (rec + r) * DP + col) = x;
+        else
+            store_out(a, b, kvh, at.row0 + wave * 32 + r, col, x);
+    }
+    if (h == 0 && q < wlive) {
+        if (at.chunks > 1) {
+            *reinterpret_cast<f32x2*>(a.part_ml + (rec + q) * 2) = f32x2{m, l};
+        } else if (a.stats) {
+            float* to = a.stats + (pair * a.rows + row) * 2;
+            to[0] = m == -INFINITY ? 0.0f : m;
+            to[1] = inv;
+        }
+    }
+}
+
+// The chunks' records of the rows whose tile has several, in their order, each
+// weighted by 2 to its maximum less the largest. Four columns a thread.
+template <int NB>
+__global__ __launch_bounds__(256) void mx4_prompt_merge_kernel(Mx4Attn a) {
+    constexpr int DP = 32 * NB, kCells = DP / 4, kRows = 256 / kCells;
+    if (static_cast<int>(threadIdx.x) >= kRows * kCells) return;
+    const int row = blockIdx.x * kRows + threadIdx.x / kCells, col = threadIdx.x % kCells * 4;
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    if (row >= a.rows) return;
+    const int tile = row / kPromptRows, row_last = min((tile + 1) * kPromptRows, a.rows) - 1;
+    const int begin = row_keys(a, a.kv, tile * kPromptRows).lo / 64, end = (row_keys(a, a.kv, row_last).hi + 63) / 64;
+    const int chunks = (end - begin + a.chunk_tiles - 1) / a.chunk_tiles;
+    if (chunks == 1) return;
+    const uint64_t pair = static_cast<uint64_t>(b) * a.kv_heads + kvh;
+    const uint64_t rec = (pair * a.row_tiles + tile) * a.chunks * kPromptRows + row % kPromptRows;
+    float top = -INFINITY;
+    for (int c = 0; c < chunks; ++c) top = fmaxf(top, a.part_ml[(rec + c * kPromptRows) * 2]);
+    const float m = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < chunks; ++c) {
+        const uint64_t r = rec + c * kPromptRows;
+        const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + r * 2);
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l += ml.y * f;
+        sum += *reinterpret_cast<const f32x4*>(a.part_o + r * DP + col) * f;
+    }
+    const float inv = 1.0f / l;
+    store_out(a, b, kvh, row, col, sum * inv);
+    if (a.stats && col == 0) {
+        a.stats[(pair * a.rows + row) * 2] = m;
+        a.stats[(pair * a.rows + row) * 2 + 1] = inv;
+    }
+}
+
 // The attention each key received, from the scores that the rows kernel kept
 // (one row tile): weights_out = weights + the sum over the rows of p. Four keys
 // a thread.
@@ -684,6 +1303,117 @@ __global__ __launch_bounds__(64 * kWeightWaves) void mx4_weights_kernel(Mx4Attn 
     }
 }
 
+// The attention each key of a prompt received, the scores taken again by the
+// same scaled products from the planes of Q and the statistics that the prompt
+// kernel left: a wave holds 32 keys and walks the tiles of 32 rows that admit one
+// of the workgroup's, whose planes the four waves share in LDS. The rows are the
+// products' columns: a lane's sixteen sums are its keys' over one column, and
+// the columns are added up at the end, in a fixed order.
+template <int NB>
+__global__ __launch_bounds__(64 * kPromptWaves) void mx4_prompt_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
+                                                                               float* weights_out, uint64_t stride) {
+    using Cfg = SumCfg<NB>;
+    constexpr int kSteps = Cfg::kSteps;
+    __shared__ __attribute__((aligned(16))) char lds[2][Cfg::kBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    const int first = blockIdx.x * (32 * kPromptWaves), base = first + wave * 32;
+    const uint64_t pair = static_cast<uint64_t>(b) * a.kv_heads + kvh;
+
+    // The rows whose queries admit a key of the workgroup.
+    const int off = a.kv - a.seq, last_key = min(first + 32 * kPromptWaves, a.kv) - 1;
+    const int i0 = a.causal ? max(0, first - off) : 0;
+    const int i1 = a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(a.seq), static_cast<int64_t>(last_key) - off + a.window)) : a.seq;
+    const int r0 = i0 * a.group / 32, r1 = (i1 * a.group + 31) / 32;
+    const char* planes = a.planes + pair * a.planes_ld * Cfg::kBytes;
+    auto fetch = [&](int t) {
+        const char* from = planes + static_cast<uint64_t>(t) * Cfg::kBytes;
+#pragma unroll
+        for (int i = 0; i < (Cfg::kBytes / 1024 + kPromptWaves - 1) / kPromptWaves; ++i) {
+            const int part = i * kPromptWaves + wave;
+            if (part < Cfg::kBytes / 1024) copy_to_lds(from + part * 1024 + lane * 16, lds[(t - r0) & 1] + part * 1024);
+        }
+    };
+    if (r0 < r1) fetch(r0);
+
+    // K: lane (key, h), step s: block 2 s + h, 16 bytes, one of each unit.
+    Frag k[kSteps];
+    uint32_t kscale = 0;
+    {
+        const uint8_t* ks = a.k + b * a.k_bs;
+        const int key = min(base + m, a.kv - 1);
+        const uint64_t g = static_cast<uint64_t>(kvh) * a.groups + key / 4;
+        const uint8_t* unit = ks + g * 64 * NB + (key % 4) * NB;
+        const uint8_t* sc = ks + a.code_bytes + g * 4 * NB + key % 4;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int p = min(2 * s + h, NB - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w |= static_cast<uint32_t>(unit[(4 * i + e) * 4 * NB + p]) << (8 * e);
+                k[s].u[i] = w;
+            }
+            kscale |= (2 * s + h < NB ? static_cast<uint32_t>(sc[4 * p]) : 127u) << (16 * s);
+        }
+    }
+    const float* stats = a.stats + pair * a.rows * 2;
+    float sum[16] = {};
+    auto row_stats = [&](int t) { return *reinterpret_cast<const f32x2*>(stats + 2 * min(32 * t + m, a.rows - 1)); };
+    f32x2 next = row_stats(r0);
+    for (int t = r0; t < r1; ++t) {
+        // This wave's part of the planes is in LDS, and the tile's statistics are
+        // in registers before the next fetch is under way.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        f32x2 st = next;
+        asm volatile("" : "+v"(st));
+        __syncthreads();
+        const int row = min(32 * t + m, a.rows - 1), row_last = min(32 * t + 31, a.rows - 1);
+        next = row_stats(t + 1);
+        if (t + 1 < r1) fetch(t + 1);
+        const Keys head = row_keys(a, a.kv, 32 * t), tail = row_keys(a, a.kv, row_last);
+        if (head.lo >= base + 32 || tail.hi <= base) continue;
+        const char* q = lds[(t - r0) & 1];
+        f32x16 c;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) c[e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const uint2 scale = *reinterpret_cast<const uint2*>(q + kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8);
+            const uint32_t ks = kscale >> (16 * s);
+            auto plane = [&](int n) { return load_plane(q + (s * kQPlanes + n) * kPlaneBytes + lane * 16); };
+            c = scaled_product<0, 1>(k[s], ks, plane(5), scale.y, c);
+            c = scaled_product<0, 0>(k[s], ks, plane(4), scale.y, c);
+            c = scaled_product<0, 3>(k[s], ks, plane(3), scale.x, c);
+            c = scaled_product<0, 2>(k[s], ks, plane(2), scale.x, c);
+            c = scaled_product<0, 1>(k[s], ks, plane(1), scale.x, c);
+            c = scaled_product<0, 0>(k[s], ks, plane(0), scale.x, c);
+        }
+        const bool whole = tail.lo <= base && head.hi >= base + 32 && 32 * t + 31 < a.rows;
+        const Keys mine = row_keys(a, a.kv, row);
+        const int lo = whole ? 0 : 32 * t + m < a.rows ? mine.lo - base : 32, hi = whole ? 32 : mine.hi - base;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int key = 8 * (e / 4) + 4 * h + e % 4;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], a.c, -st.x));
+            if (key >= lo && key < hi) sum[e] = __builtin_fmaf(p, st.y, sum[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) sum[e] += __shfl_xor(sum[e], d, 64);
+    if (m == 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int key = base + 8 * (e / 4) + 4 * h + e % 4;
+            if (key < a.kv) weights_out[pair * stride + key] = (weights ? weights[pair * stride + key] : 0.0f) + sum[e];
+        }
+    }
+}
+
 template <int NB, bool FEW>
 mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* weights, float* weights_out,
                         uint64_t stride, uint64_t kv_rows) {
@@ -727,6 +1457,74 @@ mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* 
     else
         mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(keys, 64 * kWeightWaves)), heads.y, heads.z),
                      dim3(64 * kWeightWaves), 0, a, weights, weights_out, stride);
+    return mhip::check_launch("attention (4-bit, weights)");
+}
+
+template <int NB>
+mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* weights, float* weights_out,
+                          uint64_t stride) {
+    a.row_tiles = static_cast<int>(mhip::ceil_div(a.rows, kPromptRows));
+    a.batch = static_cast<int>(batch);
+    const uint64_t pairs = batch * a.kv_heads, tiles = pairs * a.row_tiles;
+    // The key tiles of the row tiles, all and the most.
+    uint64_t units = 0, most = 0;
+    for (int t = 0; t < a.row_tiles && t < 4096; ++t) {
+        const int i0 = t * kPromptRows / a.group, i1 = (std::min((t + 1) * kPromptRows, a.rows) - 1) / a.group;
+        const int at = a.kv - a.seq;
+        const int lo = a.window > 0 ? std::max(at + i0 - (a.window - 1), 0) : 0, hi = a.causal ? at + i1 + 1 : a.kv;
+        const uint64_t n = static_cast<uint64_t>((hi + 63) / 64 - lo / 64);
+        units += n * pairs;
+        most = std::max(most, n);
+    }
+    const uint64_t slots = 2ull * ctx->compute_units;
+    a.chunks = 1;
+    a.chunk_tiles = 0;
+    a.heavy_ranks = a.row_tiles;
+    if (tiles < kSplitBelow * ctx->compute_units / 4) {
+        const uint64_t len = std::max<uint64_t>(kMinChunk, mhip::ceil_div(units, slots));
+        if (len < most) {
+            a.chunk_tiles = static_cast<int>(len);
+            a.chunks = static_cast<int>(mhip::ceil_div(most, len));
+        }
+    }
+    if (a.chunks == 1 && tiles > ctx->compute_units && tiles <= slots)
+        a.heavy_ranks = static_cast<int>(mhip::ceil_div(ctx->compute_units, pairs));
+    if (tiles * a.chunks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    const uint64_t records = a.chunks > 1 ? tiles * a.chunks * kPromptRows : 0;
+    const bool made = a.row_tiles >= kMadeFrom;
+    a.tiles_ld = mhip::ceil_div(a.kv, 64);
+    const uint64_t tile_bytes = made ? pairs * a.tiles_ld * PromptCfg<NB>::kBytes : 0;
+    a.planes_ld = static_cast<uint64_t>(a.row_tiles) * kPromptWaves;
+    const uint64_t plane_bytes = weights_out ? pairs * a.planes_ld * SumCfg<NB>::kBytes : 0;
+    const uint64_t bytes = tile_bytes + plane_bytes + records * (32 * NB + 2) * sizeof(float) + (weights_out ? pairs * a.rows * 2 * sizeof(float) : 0);
+    if (bytes) {
+        void* ws = nullptr;
+        mhip_status st = mhip::workspace(ctx, bytes, &ws);
+        if (st != MHIP_OK) return st;
+        a.tiles = static_cast<char*>(ws);
+        a.planes = weights_out ? a.tiles + tile_bytes : nullptr;
+        a.part_o = reinterpret_cast<float*>(a.tiles + tile_bytes + plane_bytes);
+        a.part_ml = a.part_o + records * (32 * NB);
+        if (weights_out) a.stats = a.part_ml + records * 2;
+    }
+    const dim3 grid(static_cast<unsigned>(tiles * a.chunks)), block(64 * kPromptWaves);
+    if (made) {
+        mhip::launch(ctx, mx4_tiles_kernel<NB>,
+                     dim3(static_cast<unsigned>(a.tiles_ld), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)), dim3(256), 0, a);
+        mhip::launch(ctx, mx4_prompt_kernel<NB, true>, grid, block, 0, a);
+    } else {
+        mhip::launch(ctx, mx4_prompt_kernel<NB, false>, grid, block, 0, a);
+    }
+    mhip_status st = mhip::check_launch("attention (4-bit, prompt)");
+    const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
+    if (st == MHIP_OK && a.chunks > 1) {
+        mhip::launch(ctx, mx4_prompt_merge_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(a.rows, 256 / (8 * NB))), heads.y, heads.z),
+                     dim3(256), 0, a);
+        st = mhip::check_launch("attention (4-bit, prompt merge)");
+    }
+    if (st != MHIP_OK || !weights_out) return st;
+    mhip::launch(ctx, mx4_prompt_weights_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(a.kv, 32 * kPromptWaves)), heads.y, heads.z),
+                 block, 0, a, weights, weights_out, stride);
     return mhip::check_launch("attention (4-bit, weights)");
 }
 
@@ -801,6 +1599,7 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     a.causal = p->causal ? 1 : 0;
     a.window = p->window_size > 0 ? static_cast<int>(std::min<int64_t>(p->window_size, 1LL << 30)) : -1;
     a.vec = d % 4 == 0 && mhip::aligned16(out) && a.o_bs % 4 == 0;
+    a.vec_q = d % 4 == 0 && mhip::aligned16(q) && a.q_bs % 4 == 0;
     const float scale = p->scale > 0.0f ? p->scale : 1.0f / std::sqrt(static_cast<float>(d));
     a.c = scale * kLog2e;
     if (p->bounded_key_count) {
@@ -811,6 +1610,15 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     }
     const uint64_t plan_rows = p->bounded_key_count ? p->kv_rows : p->kv_seq_len;
     const bool few = a.rows <= kRowTile<true>;
+    if (p->seq_len > 1 && rows >= 64) {
+        switch (mhip::mx4_blocks(d)) {
+            case 1: return launch_prompt<1>(ctx, a, batch, weights, weights_out, p->kv_rows);
+            case 2: return launch_prompt<2>(ctx, a, batch, weights, weights_out, p->kv_rows);
+            case 3: return launch_prompt<3>(ctx, a, batch, weights, weights_out, p->kv_rows);
+            case 4: return launch_prompt<4>(ctx, a, batch, weights, weights_out, p->kv_rows);
+            default: break;
+        }
+    }
     switch (mhip::mx4_blocks(d)) {
         case 1:
             return few ? launch_rows<1, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
