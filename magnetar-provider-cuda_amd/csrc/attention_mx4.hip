@@ -63,8 +63,6 @@ struct Mx4Attn {
     int vec_q;                    // rows of q are whole float4s
     int row_tiles, heavy_ranks, chunks, chunk_tiles, batch;
     float c;                      // scale * log2(e)
-    char* tiles;                  // [batch][kv head][tile] PromptCfg::kBytes
-    uint64_t tiles_ld;
     char* planes;                 // [batch][kv head][32 rows] SumCfg::kBytes (weights asked for)
     uint64_t planes_ld;
     float* part_o;                // [batch][kv head][row tile][chunk][row][DP]
@@ -319,7 +317,6 @@ __device__ __forceinline__ uint64_t row_at(const Mx4Attn& a, int kvh, int row) {
     return static_cast<uint64_t>(i) * a.q_ld + static_cast<uint64_t>(head) * a.d;
 }
 
-constexpr int kWeightWaves = 4;
 constexpr int kMaxChunks = 256;
 // Waves of a rows workgroup: eight, of a head of more than four blocks four
 // (their sums in LDS are 16 rows a wave).
@@ -636,12 +633,11 @@ __device__ __forceinline__ f32x16 mfma32(const Frag& a, const Frag& b, f32x16 c)
 // 1.4e-7, six 3.0e-8; with one value of a block 1000 times the others and keys
 // that are zero there, 2.6e-5 and 7.9e-7.)
 constexpr int kQPlanes = 6;
-template <int NB, bool MADE>
+template <int NB>
 struct QPlanes {
     static constexpr int kSteps = (NB + 1) / 2;  // of two blocks, one a half of the wave
-    // Above two blocks, with the units that a thread carries, the registers do not
-    // hold all: planes 3 to 5 stay in LDS.
-    static constexpr bool kLow = NB > 2 && !MADE;
+    // Above two blocks the registers do not hold all: planes 3 to 5 stay in LDS.
+    static constexpr bool kLow = NB > 2;
     u32x6 f[kSteps][kQPlanes];
     uint32_t scale[kSteps][2];  // scale bytes of planes 0-3 and 4-5
 };
@@ -664,10 +660,10 @@ __device__ __forceinline__ u32x6 load_plane(const char* p) {
 // Lane (row, h), step s: block 2 s + h of the row (32 NB values in LDS, zeros
 // past d), its values 2 i and 2 i + 1 the block's columns i and 16 + i, as the
 // codes of K lie.
-template <int NB, bool MADE>
-__device__ __forceinline__ void make_q_planes(const float* qrow, int h, QPlanes<NB, MADE>& q) {
+template <int NB>
+__device__ __forceinline__ void make_q_planes(const float* qrow, int h, QPlanes<NB>& q) {
 #pragma unroll
-    for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s) {
+    for (int s = 0; s < QPlanes<NB>::kSteps; ++s) {
         const int p = 2 * s + h;
         f32x16 lo, hi;
         uint32_t top = 0;
@@ -729,13 +725,13 @@ __device__ __forceinline__ f32x16 scaled_product(const Frag& k, uint32_t kscale,
 }
 // st[0] and st[1] (two chains) += 32 keys each by all planes of Q, the smallest
 // first. `low`: planes 3 to 5 of the step, from LDS.
-template <int OPK, int NB, bool MADE>
-__device__ __forceinline__ void score_step(const Frag& k0, const Frag& k1, uint32_t s0, uint32_t s1, const QPlanes<NB, MADE>& q, int s,
+template <int OPK, int NB>
+__device__ __forceinline__ void score_step(const Frag& k0, const Frag& k1, uint32_t s0, uint32_t s1, const QPlanes<NB>& q, int s,
                                            const char* low, f32x16 (&st)[2]) {
     u32x6 f[3];
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
-        if constexpr (QPlanes<NB, MADE>::kLow)
+        if constexpr (QPlanes<NB>::kLow)
             f[n] = load_plane(low + (3 * s + n) * kPlaneBytes);
         else
             f[n] = q.f[s][3 + n];
@@ -754,17 +750,7 @@ __device__ __forceinline__ void score_step(const Frag& k0, const Frag& k1, uint3
     st[1] = scaled_product<OPK, 0>(k1, s1, q.f[s][0], q.scale[s][0], st[1]);
 }
 
-#ifndef SB
-#define SB 4
-#endif
-#ifndef MC
-#define MC 8
-#endif
-constexpr uint64_t kSplitBelow = SB, kMinChunk = MC;
-#ifndef MF
-#define MF 4
-#endif
-constexpr int kMadeFrom = MF;
+constexpr uint64_t kMinChunk = 8;  // key tiles
 constexpr float kLag = 8.0f;
 constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 
@@ -774,22 +760,22 @@ constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 //   K as codes, [half of 32 keys][block][key] 16 bytes (the blocks 16 bytes
 //     apart in the banks). A unit has one byte of each of 4 NB (key, block)
 //     pairs; four lanes transpose theirs to write four bytes of a pair at once.
-//     Behind them a key's scale bytes, a dword a key.
+//     Behind them a key's scale bytes, a dword for four blocks.
 //   V as bf16 operands of 32x32x16 products, [half][step of 16 keys][block][lane]
 //     16 bytes, lane (m, h) the keys 4 h to 4 h + 3 and 8 + 4 h to 11 + 4 h of
 //     column m of the block: the keys whose weights that half of the wave has
 //     after the scores.
-template <int NB, bool MADE = true>
+template <int NB>
 struct PromptCfg {
     static constexpr int kBlock = 32 * 16 + 16;
-    static constexpr int kKHalf = NB * kBlock + 128;  // codes, scales
+    static constexpr int kWords = (NB + 3) / 4;  // of a key's scale bytes
+    static constexpr int kKHalf = NB * kBlock + 128 * kWords;  // codes, scales
     static constexpr int kVHalf = 2 * NB * 1024;
-    static constexpr int kNan = 2 * (kKHalf + kVHalf);  // behind the tile: its NaN bits, [block][half]
-    static constexpr int kBytes = (kNan + 8 * NB + 1023) / 1024 * 1024;
+    static constexpr int kBytes = 2 * (kKHalf + kVHalf);  // of a tile
     // A wave's rows of q or of the output pass through LDS, 16 bytes apart in
     // the banks, so that memory is read and written along the rows.
     static constexpr int kRow = 32 * NB + 4;  // floats
-    static constexpr int kLowBytes = QPlanes<NB, MADE>::kLow ? 3 * QPlanes<NB, MADE>::kSteps * kPlaneBytes : 0;  // a wave
+    static constexpr int kLowBytes = QPlanes<NB>::kLow ? 3 * QPlanes<NB>::kSteps * kPlaneBytes : 0;  // a wave
     static constexpr int kLoop = 2 * kBytes + kPromptWaves * kLowBytes, kRows = kPromptWaves * 32 * kRow * 4;
     static constexpr int kLds = kLoop > kRows ? kLoop : kRows;
 };
@@ -837,10 +823,16 @@ __device__ __forceinline__ void store_keys(const Carry<NB>& c, char* lds, int kg
         const int at = 4 * w + lane4, i = at / NB, p = at % NB;
         *reinterpret_cast<uint32_t*>(kd + p * Cfg::kBlock + (4 * j + i) * 16 + (n & ~3)) = y;
     }
-    uint32_t s = 0;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) s |= (p < NB ? c.ks.w[p < NB ? p : 0] >> (8 * lane4) & 255u : 127u) << (8 * p);
-    if (n < 4) *reinterpret_cast<uint32_t*>(kd + NB * Cfg::kBlock + (4 * j + n) * 4) = s;
+    for (int w = 0; w < Cfg::kWords; ++w) {
+        uint32_t s = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int p = 4 * w + e;
+            s |= (p < NB ? c.ks.w[p < NB ? p : 0] >> (8 * lane4) & 255u : 127u) << (8 * e);
+        }
+        if (n < 4) *reinterpret_cast<uint32_t*>(kd + NB * Cfg::kBlock + w * 128 + (4 * j + n) * 4) = s;
+    }
 }
 
 // `nan`: a tile's keys of each block whose value is no number, a bit a key.
@@ -891,16 +883,20 @@ __device__ __forceinline__ Frag lds_frag(const char* p) {
 
 // S^T of a tile's 64 keys by the wave's 32 rows: st[kk][r] is key 32 kk + 8 (r /
 // 4) + 4 h + r % 4 of row lane % 32.
-template <int NB, bool MADE>
-__device__ __forceinline__ void tile_scores(const char* kt, const QPlanes<NB, MADE>& q, const char* low, int m, int h, f32x16 (&st)[2]) {
+template <int NB>
+__device__ __forceinline__ void tile_scores(const char* kt, const QPlanes<NB>& q, const char* low, int m, int h, f32x16 (&st)[2]) {
     using Cfg = PromptCfg<NB>;
     const char* k0 = kt;
     const char* k1 = kt + Cfg::kKHalf;
-    const uint32_t scale0 = *reinterpret_cast<const uint32_t*>(k0 + NB * Cfg::kBlock + m * 4) >> (8 * h);
-    const uint32_t scale1 = *reinterpret_cast<const uint32_t*>(k1 + NB * Cfg::kBlock + m * 4) >> (8 * h);
+    uint32_t scale0[Cfg::kWords], scale1[Cfg::kWords];
+#pragma unroll
+    for (int w = 0; w < Cfg::kWords; ++w) {
+        scale0[w] = *reinterpret_cast<const uint32_t*>(k0 + NB * Cfg::kBlock + w * 128 + m * 4) >> (8 * h);
+        scale1[w] = *reinterpret_cast<const uint32_t*>(k1 + NB * Cfg::kBlock + w * 128 + m * 4) >> (8 * h);
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) st[0][e] = st[1][e] = 0.0f;
-    constexpr int kSteps = QPlanes<NB, MADE>::kSteps;
+    constexpr int kSteps = QPlanes<NB>::kSteps;
     Frag k[kSteps][2];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -908,8 +904,13 @@ __device__ __forceinline__ void tile_scores(const char* kt, const QPlanes<NB, MA
         k[i][0] = lds_frag(k0 + at);
         k[i][1] = lds_frag(k1 + at);
     }
-    score_step<0>(k[0][0], k[0][1], scale0, scale1, q, 0, low, st);
-    if constexpr (kSteps > 1) score_step<2>(k[1][0], k[1][1], scale0, scale1, q, 1, low, st);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        if (i % 2 == 0)
+            score_step<0>(k[i][0], k[i][1], scale0[i / 2], scale1[i / 2], q, i, low, st);
+        else
+            score_step<2>(k[i][0], k[i][1], scale0[i / 2], scale1[i / 2], q, i, low, st);
+    }
 }
 
 // 16 bytes a lane from memory to 1024 bytes of LDS, whose address is the
@@ -959,30 +960,9 @@ __device__ __forceinline__ PromptPlace prompt_place(const Mx4Attn& a, int block)
     return w;
 }
 
-// The tiles of a KV head as the workgroups' LDS takes them, made once where
-// several workgroups read each: [sequence][KV head][tile] kBytes.
 template <int NB>
-__global__ __launch_bounds__(256) void mx4_tiles_kernel(Mx4Attn a) {
+__global__ __launch_bounds__(64 * kPromptWaves, NB > 4 ? 1 : 2) void mx4_prompt_kernel(Mx4Attn a) {
     using Cfg = PromptCfg<NB>;
-    __shared__ __attribute__((aligned(16))) char lds[Cfg::kBytes];
-    const int tid = threadIdx.x, kg = tid >> 4, n = tid & 15;
-    const int t = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-    uint32_t(*nan)[2] = reinterpret_cast<uint32_t(*)[2]>(lds + Cfg::kNan);
-    if (tid < 2 * NB) (&nan[0][0])[tid] = 0;
-    Carry<NB> c;
-    load_carry<NB>(a, b, kvh, t, kg, n, c);
-    __syncthreads();
-    take_nan<NB>(c, nan, kg, n);
-    store_keys<NB>(c, lds, kg, n);
-    store_values<NB>(c, lds, kg, n);
-    __syncthreads();
-    uint4* to = reinterpret_cast<uint4*>(a.tiles + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.tiles_ld + t) * Cfg::kBytes);
-    for (int i = tid; i < (Cfg::kNan + 8 * NB + 15) / 16; i += 256) to[i] = reinterpret_cast<const uint4*>(lds)[i];
-}
-
-template <int NB, bool MADE>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Attn a) {
-    using Cfg = PromptCfg<NB, MADE>;
     constexpr int DP = 32 * NB;
     __shared__ __attribute__((aligned(16))) char lds[Cfg::kLds];
     __shared__ uint32_t nan[3][NB][2];
@@ -998,19 +978,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Att
     const Keys mine = row_keys(a, a.kv, row);
     const Keys whead = row_keys(a, a.kv, wrow0), wtail = row_keys(a, a.kv, wrow_last);
 
-    // MADE: the tiles come as they are, straight to LDS; else from the stores.
     Carry<NB> carry;
-    const char* made = MADE ? a.tiles + (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.tiles_ld * Cfg::kBytes : nullptr;
-    auto fetch = [&](int t, char* to) {
-        const char* from = made + static_cast<uint64_t>(t) * Cfg::kBytes;
-#pragma unroll
-        for (int i = 0; i < (Cfg::kBytes / 1024 + kPromptWaves - 1) / kPromptWaves; ++i) {
-            const int part = i * kPromptWaves + wave;
-            if (part < Cfg::kBytes / 1024)
-                copy_to_lds(from + part * 1024 + lane * 16, to + part * 1024);
-        }
-    };
-    if (!MADE) load_carry<NB>(a, b, kvh, t0, kg, n, carry);
+    load_carry<NB>(a, b, kvh, t0, kg, n, carry);
     float* wrows = reinterpret_cast<float*>(lds) + wave * 32 * Cfg::kRow;
     for (int u = lane; u < 8 * DP; u += 64) {
         const int r = u / (DP / 4), col = u % (DP / 4) * 4;
@@ -1019,32 +988,19 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Att
     }
     if (tid < 6 * NB) (&nan[0][0][0])[tid] = 0;
     __syncthreads();
-    QPlanes<NB, MADE> qp;
-    make_q_planes<NB, MADE>(wrows + q * Cfg::kRow, h, qp);
+    QPlanes<NB> qp;
+    make_q_planes<NB>(wrows + q * Cfg::kRow, h, qp);
     __syncthreads();
     char* low = lds + 2 * Cfg::kBytes + wave * Cfg::kLowBytes + lane * 16;
-    if (a.planes && at.chunk == 0 && wave_live) {
-        char* keep = a.planes + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.planes_ld + at.tile * kPromptWaves + wave) * SumCfg<NB>::kBytes;
+    if constexpr (QPlanes<NB>::kLow)
 #pragma unroll
-        for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s) {
-#pragma unroll
-            for (int n = 0; n < kQPlanes; ++n) store_plane(keep + (s * kQPlanes + n) * kPlaneBytes + lane * 16, qp.f[s][n]);
-            *reinterpret_cast<uint2*>(keep + QPlanes<NB, MADE>::kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8) = uint2{qp.scale[s][0], qp.scale[s][1]};
-        }
-    }
-    if constexpr (QPlanes<NB, MADE>::kLow)
-#pragma unroll
-        for (int s = 0; s < QPlanes<NB, MADE>::kSteps; ++s)
+        for (int s = 0; s < QPlanes<NB>::kSteps; ++s)
 #pragma unroll
             for (int n = 0; n < 3; ++n) store_plane(low + (3 * s + n) * kPlaneBytes, qp.f[s][3 + n]);
-    if constexpr (MADE) {
-        fetch(t0, lds);
-    } else {
-        take_nan<NB>(carry, nan[0], kg, n);
-        store_keys<NB>(carry, lds, kg, n);
-        store_values<NB>(carry, lds, kg, n);
-        load_carry<NB>(a, b, kvh, t0 + 1, kg, n, carry);
-    }
+    take_nan<NB>(carry, nan[0], kg, n);
+    store_keys<NB>(carry, lds, kg, n);
+    store_values<NB>(carry, lds, kg, n);
+    load_carry<NB>(a, b, kvh, t0 + 1, kg, n, carry);
 
     f32x16 o[NB];
 #pragma unroll
@@ -1055,32 +1011,24 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Att
     int slot = 0;  // (t - t0) % 3
     for (int t = t0; t < t1; ++t) {
         const int base = 64 * t, next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-        if (MADE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile is in LDS
         __syncthreads();
-        if (!MADE && tid < 2 * NB) (&nan[after][0][0])[tid] = 0;
+        if (tid < 2 * NB) (&nan[after][0][0])[tid] = 0;
         const char* kt = lds + ((t - t0) & 1) * Cfg::kBytes;
         const char* vt = kt + 2 * Cfg::kKHalf;
         char* to = lds + ((t + 1 - t0) & 1) * Cfg::kBytes;
-        if constexpr (MADE) {
-            if (t + 1 < t1) fetch(t + 1, to);
-        } else {
-            take_nan<NB>(carry, nan[next], kg, n);
-        }
         if (!(wave_live && base < wtail.hi && base + 64 > whead.lo)) {
-            if constexpr (!MADE) {
-                store_keys<NB>(carry, to, kg, n);
-                store_values<NB>(carry, to, kg, n);
-                load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
-            }
+            take_nan<NB>(carry, nan[next], kg, n);
+            store_keys<NB>(carry, to, kg, n);
+            store_values<NB>(carry, to, kg, n);
+            load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
         } else {
             f32x16 st[2];
-            const uint32_t no_number = any_nan(MADE ? reinterpret_cast<const uint32_t*>(kt + Cfg::kNan) : &nan[slot][0][0], 2 * NB);
-            tile_scores<NB, MADE>(kt, qp, low, q, h, st);
-            if constexpr (!MADE) {
-                store_keys<NB>(carry, to, kg, n);
-                store_values<NB>(carry, to, kg, n);
-                load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
-            }
+            const uint32_t no_number = any_nan(&nan[slot][0][0], 2 * NB);
+            tile_scores<NB>(kt, qp, low, q, h, st);
+            take_nan<NB>(carry, nan[next], kg, n);
+            store_keys<NB>(carry, to, kg, n);
+            store_values<NB>(carry, to, kg, n);
+            load_carry<NB>(a, b, kvh, t + 2, kg, n, carry);
             if (base < wtail.lo || base + 64 > whead.hi) {
                 asm volatile("");  // a branch: 96 instructions that few tiles need
 #pragma unroll
@@ -1135,7 +1083,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void mx4_prompt_kernel(Mx4Att
                 asm volatile("");  // a branch
 #pragma unroll
                 for (int c = 0; c < NB; ++c) {
-                    const uint32_t* flags = MADE ? reinterpret_cast<const uint32_t*>(kt + Cfg::kNan) + 2 * c : nan[slot][c];
+                    const uint32_t* flags = nan[slot][c];
                     const uint64_t bad = static_cast<uint64_t>(flags[1]) << 32 | flags[0];
                     const int lo = min(max(mine.lo - base, 0), 64), hi = min(max(mine.hi - base, 0), 64);
                     const uint64_t mask = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
@@ -1243,106 +1191,78 @@ __global__ __launch_bounds__(256) void mx4_kept_weights_kernel(Mx4Attn a, const 
         if (key + x < kv) weights_out[at + x] = (weights ? weights[at + x] : 0.0f) + sum[x];
 }
 
-// The same for any number of rows, the scores taken again from the rows'
-// statistics. A
-// wave takes 64 keys and every row tile that admits one of them.
+// The planes of Q for the weights' kernel: a wave 32 rows, by way of LDS.
 template <int NB>
-__global__ __launch_bounds__(64 * kWeightWaves) void mx4_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
-                                                                  float* weights_out, uint64_t stride) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const int kv = a.kv + (a.advance ? static_cast<int>(*a.advance) : 0);
-    const int base = (blockIdx.x * kWeightWaves + wave) * 64;
-    if (base >= kv) return;
-    const uint8_t* ks = a.k + b * a.k_bs;
-    const uint64_t head_units = static_cast<uint64_t>(kvh) * a.groups;
-    const uint32_t* kc = reinterpret_cast<const uint32_t*>(ks) + head_units * 16 * NB;
-    const uint32_t* kx = reinterpret_cast<const uint32_t*>(ks + a.code_bytes) + head_units * NB;
-    Strip<NB> k;
-    load_k<NB>(kc, kx, base / 4, (kv - 1) / 4, n, g, k);
-    float sum[4][4] = {};
-    // The first query that admits a key of the strip, and the last.
-    int i0 = 0, i1 = a.seq;
-    if (a.causal) i0 = max(0, base - (kv - a.seq));
-    if (a.window > 0) i1 = static_cast<int>(min(static_cast<int64_t>(a.seq), static_cast<int64_t>(base) + 63 - (kv - a.seq) + a.window));
-    const float* stats = a.stats + (static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.rows * 2;
-    for (int tile = i0 * a.group / 16; tile * 16 < i1 * a.group; ++tile) {
-        const int row = min(tile * 16 + n, a.rows - 1);
-        Rows<false> q[NB];
-        load_q<NB, false>(a, a.q + b * a.q_bs + row_at(a, kvh, row), g, Plane{}, q);
-        f32x4 st[4];
-        scores<NB, false>(k, q, st);
-        const Keys mine = row_keys(a, kv, row);
-        const float m = stats[2 * row], inv = stats[2 * row + 1];
-        const bool live = tile * 16 + n < a.rows;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = base + 16 * g + 4 * r + i;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i][r], a.c, -m)) * inv;
-                if (live && key >= mine.lo && key < mine.hi) sum[i][r] += p;
-            }
+__global__ __launch_bounds__(64) void mx4_planes_kernel(Mx4Attn a) {
+    constexpr int DP = 32 * NB, kRow = PromptCfg<NB>::kRow;
+    __shared__ float rows[32 * kRow];
+    const int lane = threadIdx.x, tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    for (int u = lane; u < 8 * DP; u += 64) {
+        const int r = u / (DP / 4), col = u % (DP / 4) * 4;
+        const int from = min(tile * 32 + r, a.rows - 1);
+        *reinterpret_cast<f32x4*>(rows + r * kRow + col) = load_q4(a, a.q + b * a.q_bs + row_at(a, kvh, from), col);
     }
+    __syncthreads();
+    QPlanes<NB> q;
+    make_q_planes<NB>(rows + (lane & 31) * kRow, lane >> 5, q);
+    char* to = a.planes + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.planes_ld + tile) * SumCfg<NB>::kBytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int s = 0; s < QPlanes<NB>::kSteps; ++s) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int off = 1; off < 16; off *= 2) sum[i][r] += __shfl_xor(sum[i][r], off, 64);
-    if (n == 0) {
-        const uint64_t at = (static_cast<uint64_t>(b) * a.kv_heads + kvh) * stride;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = base + 16 * g + 4 * r + i;
-                if (key < kv) weights_out[at + key] = (weights ? weights[at + key] : 0.0f) + sum[i][r];
-            }
+        for (int n = 0; n < kQPlanes; ++n) store_plane(to + (s * kQPlanes + n) * kPlaneBytes + lane * 16, q.f[s][n]);
+        *reinterpret_cast<uint2*>(to + QPlanes<NB>::kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8) = uint2{q.scale[s][0], q.scale[s][1]};
     }
 }
 
-// The attention each key of a prompt received, the scores taken again by the
-// same scaled products from the planes of Q and the statistics that the prompt
-// kernel left: a wave holds 32 keys and walks the tiles of 32 rows that admit one
-// of the workgroup's, whose planes the four waves share in LDS. The rows are the
-// products' columns: a lane's sixteen sums are its keys' over one column, and
-// the columns are added up at the end, in a fixed order.
+// The attention each key received from any number of rows, the scores taken
+// again by the prompts' scaled products from the planes of Q and the statistics
+// that the attention left: a wave holds 64 keys and walks the tiles of 32 rows that admit one
+// of the workgroup's (its share of them, of `chunks`), whose planes the four
+// waves share in LDS. The rows are the products' columns: a lane's sums are its
+// keys' over one column, and the columns are added up at the end, in a fixed
+// order; so are the chunks' sums, by mx4_sum_weights_kernel.
+constexpr int kSumKeys = 64 * kPromptWaves, kSumRows = 8;
 template <int NB>
-__global__ __launch_bounds__(64 * kPromptWaves) void mx4_prompt_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
-                                                                               float* weights_out, uint64_t stride) {
+__global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn a, const float* __restrict__ weights,
+                                                                               float* weights_out, uint64_t stride, int chunks,
+                                                                        float* part, uint64_t part_ld) {
     using Cfg = SumCfg<NB>;
+    if (a.advance) a.kv += static_cast<int>(*a.advance);
     constexpr int kSteps = Cfg::kSteps;
     __shared__ __attribute__((aligned(16))) char lds[2][Cfg::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.y, b = blockIdx.z;
-    const int first = blockIdx.x * (32 * kPromptWaves), base = first + wave * 32;
+    const int block = chunks > 1 ? blockIdx.x / chunks : blockIdx.x, chunk = chunks > 1 ? blockIdx.x % chunks : 0;
+    const int first = block * kSumKeys, base = first + wave * 64;
+    if (first >= a.kv) return;
     const uint64_t pair = static_cast<uint64_t>(b) * a.kv_heads + kvh;
 
-    // The rows whose queries admit a key of the workgroup.
-    const int off = a.kv - a.seq, last_key = min(first + 32 * kPromptWaves, a.kv) - 1;
+    // The rows whose queries admit a key of the workgroup, the chunk's share.
+    const int off = a.kv - a.seq, last_key = min(first + kSumKeys, a.kv) - 1;
     const int i0 = a.causal ? max(0, first - off) : 0;
     const int i1 = a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(a.seq), static_cast<int64_t>(last_key) - off + a.window)) : a.seq;
-    const int r0 = i0 * a.group / 32, r1 = (i1 * a.group + 31) / 32;
+    const int begin = i0 * a.group / 32, end = max((i1 * a.group + 31) / 32, begin), per = (end - begin + chunks - 1) / chunks;
+    const int r0 = min(begin + chunk * per, end), r1 = min(r0 + per, end);
     const char* planes = a.planes + pair * a.planes_ld * Cfg::kBytes;
     auto fetch = [&](int t) {
         const char* from = planes + static_cast<uint64_t>(t) * Cfg::kBytes;
 #pragma unroll
         for (int i = 0; i < (Cfg::kBytes / 1024 + kPromptWaves - 1) / kPromptWaves; ++i) {
-            const int part = i * kPromptWaves + wave;
-            if (part < Cfg::kBytes / 1024) copy_to_lds(from + part * 1024 + lane * 16, lds[(t - r0) & 1] + part * 1024);
+            const int p = i * kPromptWaves + wave;
+            if (p < Cfg::kBytes / 1024) copy_to_lds(from + p * 1024 + lane * 16, lds[(t - r0) & 1] + p * 1024);
         }
     };
     if (r0 < r1) fetch(r0);
 
-    // K: lane (key, h), step s: block 2 s + h, 16 bytes, one of each unit.
-    Frag k[kSteps];
-    uint32_t kscale = 0;
-    {
+    // K, halves of 32 keys: lane (key, h), step s: block 2 s + h, 16 bytes, one of
+    // each unit.
+    Frag k[2][kSteps];
+    uint32_t kscale[2][(kSteps + 1) / 2] = {};
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
         const uint8_t* ks = a.k + b * a.k_bs;
-        const int key = min(base + m, a.kv - 1);
+        const int key = min(base + 32 * kk + m, a.kv - 1);
         const uint64_t g = static_cast<uint64_t>(kvh) * a.groups + key / 4;
         const uint8_t* unit = ks + g * 64 * NB + (key % 4) * NB;
         const uint8_t* sc = ks + a.code_bytes + g * 4 * NB + key % 4;
@@ -1354,13 +1274,13 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_prompt_weights_kernel(M
                 uint32_t w = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w |= static_cast<uint32_t>(unit[(4 * i + e) * 4 * NB + p]) << (8 * e);
-                k[s].u[i] = w;
+                k[kk][s].u[i] = w;
             }
-            kscale |= (2 * s + h < NB ? static_cast<uint32_t>(sc[4 * p]) : 127u) << (16 * s);
+            kscale[kk][s / 2] |= (2 * s + h < NB ? static_cast<uint32_t>(sc[4 * p]) : 127u) << (16 * (s % 2));
         }
     }
     const float* stats = a.stats + pair * a.rows * 2;
-    float sum[16] = {};
+    float sum[2][16] = {};
     auto row_stats = [&](int t) { return *reinterpret_cast<const f32x2*>(stats + 2 * min(32 * t + m, a.rows - 1)); };
     f32x2 next = row_stats(r0);
     for (int t = r0; t < r1; ++t) {
@@ -1374,44 +1294,125 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_prompt_weights_kernel(M
         next = row_stats(t + 1);
         if (t + 1 < r1) fetch(t + 1);
         const Keys head = row_keys(a, a.kv, 32 * t), tail = row_keys(a, a.kv, row_last);
-        if (head.lo >= base + 32 || tail.hi <= base) continue;
+        if (head.lo >= base + 64 || tail.hi <= base) continue;
         const char* q = lds[(t - r0) & 1];
-        f32x16 c;
+        f32x16 c[2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) c[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) c[0][e] = c[1][e] = 0.0f;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint2 scale = *reinterpret_cast<const uint2*>(q + kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8);
-            const uint32_t ks = kscale >> (16 * s);
-            auto plane = [&](int n) { return load_plane(q + (s * kQPlanes + n) * kPlaneBytes + lane * 16); };
-            c = scaled_product<0, 1>(k[s], ks, plane(5), scale.y, c);
-            c = scaled_product<0, 0>(k[s], ks, plane(4), scale.y, c);
-            c = scaled_product<0, 3>(k[s], ks, plane(3), scale.x, c);
-            c = scaled_product<0, 2>(k[s], ks, plane(2), scale.x, c);
-            c = scaled_product<0, 1>(k[s], ks, plane(1), scale.x, c);
-            c = scaled_product<0, 0>(k[s], ks, plane(0), scale.x, c);
+            const uint32_t s0 = kscale[0][s / 2] >> (16 * (s % 2)), s1 = kscale[1][s / 2] >> (16 * (s % 2));
+            auto both = [&](auto opq, int n, uint32_t qs) {
+                const u32x6 f = load_plane(q + (s * kQPlanes + n) * kPlaneBytes + lane * 16);
+                c[0] = scaled_product<0, decltype(opq)::value>(k[0][s], s0, f, qs, c[0]);
+                c[1] = scaled_product<0, decltype(opq)::value>(k[1][s], s1, f, qs, c[1]);
+            };
+            both(std::integral_constant<int, 1>{}, 5, scale.y);
+            both(std::integral_constant<int, 0>{}, 4, scale.y);
+            both(std::integral_constant<int, 3>{}, 3, scale.x);
+            both(std::integral_constant<int, 2>{}, 2, scale.x);
+            both(std::integral_constant<int, 1>{}, 1, scale.x);
+            both(std::integral_constant<int, 0>{}, 0, scale.x);
         }
-        const bool whole = tail.lo <= base && head.hi >= base + 32 && 32 * t + 31 < a.rows;
-        const Keys mine = row_keys(a, a.kv, row);
-        const int lo = whole ? 0 : 32 * t + m < a.rows ? mine.lo - base : 32, hi = whole ? 32 : mine.hi - base;
+        if (tail.lo <= base && head.hi >= base + 64 && 32 * t + 31 < a.rows) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int key = 8 * (e / 4) + 4 * h + e % 4;
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[e], a.c, -st.x));
-            if (key >= lo && key < hi) sum[e] = __builtin_fmaf(p, st.y, sum[e]);
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sum[kk][e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(c[kk][e], a.c, -st.x)), st.y, sum[kk][e]);
+        } else {
+            Keys mine = row_keys(a, a.kv, row);
+            if (32 * t + m >= a.rows) mine.hi = mine.lo;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(c[kk][e], a.c, -st.x));
+                    if (!outside(mine, base + 32 * kk + 8 * (e / 4) + 4 * h + e % 4)) sum[kk][e] = __builtin_fmaf(p, st.y, sum[kk][e]);
+                }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) sum[e] += __shfl_xor(sum[e], d, 64);
-    if (m == 0) {
+        for (int e = 0; e < 16; ++e)
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) sum[kk][e] += __shfl_xor(sum[kk][e], d, 64);
+    if (m != 0) return;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int key = base + 8 * (e / 4) + 4 * h + e % 4;
-            if (key < a.kv) weights_out[pair * stride + key] = (weights ? weights[pair * stride + key] : 0.0f) + sum[e];
+            const int key = base + 32 * kk + 8 * (e / 4) + 4 * h + e % 4;
+            if (key >= a.kv) continue;
+            if (chunks > 1)
+                part[(pair * chunks + chunk) * part_ld + key] = sum[kk][e];
+            else
+                weights_out[pair * stride + key] = (weights ? weights[pair * stride + key] : 0.0f) + sum[kk][e];
         }
+}
+
+// The chunks' sums of a key, in their order.
+__global__ __launch_bounds__(256) void mx4_sum_weights_kernel(Mx4Attn a, const float* __restrict__ part, uint64_t part_ld, int chunks,
+                                                              const float* __restrict__ weights, float* weights_out, uint64_t stride) {
+    const int key = blockIdx.x * 256 + threadIdx.x;
+    if (key >= a.kv + (a.advance ? static_cast<int>(*a.advance) : 0)) return;
+    const uint64_t pair = static_cast<uint64_t>(blockIdx.z) * a.kv_heads + blockIdx.y;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) sum += part[(pair * chunks + c) * part_ld + key];
+    weights_out[pair * stride + key] = (weights ? weights[pair * stride + key] : 0.0f) + sum;
+}
+
+struct KeyTiles {
+    uint64_t all = 0, most = 0;
+};
+// The key tiles that the prompts' row tiles of one KV head see, all together and
+// the most of one. (Of very long prompts the first 4096 row tiles: neither the
+// choice of a kernel nor a split hangs on the rest.)
+KeyTiles key_tiles(const Mx4Attn& a) {
+    KeyTiles k;
+    for (int row = 0, t = 0; row < a.rows && t < 4096; row += kPromptRows, ++t) {
+        const int i0 = row / a.group, i1 = (std::min(row + kPromptRows, a.rows) - 1) / a.group, at = a.kv - a.seq;
+        const int lo = a.window > 0 ? std::max(at + i0 - (a.window - 1), 0) : 0, hi = a.causal ? at + i1 + 1 : a.kv;
+        const uint64_t n = static_cast<uint64_t>((hi + 63) / 64 - lo / 64);
+        k.all += n;
+        k.most = std::max(k.most, n);
     }
+    return k;
+}
+
+// How the weights of more than one row tile are taken: the scratch (planes and
+// chunks' sums, 16-byte multiples) and the launches.
+struct SumPlan {
+    uint64_t keys = 0, key_blocks = 0, chunks = 1, plane_bytes = 0, part_bytes = 0;
+};
+template <int NB>
+SumPlan sum_plan(mhip_ctx* ctx, Mx4Attn& a, uint64_t pairs, uint64_t kv_rows) {
+    SumPlan p;
+    p.keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
+    const uint64_t row_blocks = mhip::ceil_div(a.rows, 32);
+    a.planes_ld = row_blocks;
+    // Four workgroups for each CU, of at least eight row tiles.
+    p.key_blocks = mhip::ceil_div(p.keys, kSumKeys);
+    p.chunks = std::max<uint64_t>(1, std::min(mhip::ceil_div(4ull * ctx->compute_units, p.key_blocks * pairs), row_blocks / kSumRows));
+    p.plane_bytes = pairs * row_blocks * SumCfg<NB>::kBytes;
+    p.part_bytes = p.chunks > 1 ? (pairs * p.chunks * p.keys * sizeof(float) + 15) / 16 * 16 : 0;
+    return p;
+}
+template <int NB>
+mhip_status launch_weights(mhip_ctx* ctx, const Mx4Attn& a, uint64_t batch, const SumPlan& p, float* part, const float* weights,
+                           float* weights_out, uint64_t stride) {
+    const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
+    if (p.key_blocks * p.chunks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    mhip::launch(ctx, mx4_planes_kernel<NB>, dim3(static_cast<unsigned>(a.planes_ld), heads.y, heads.z), dim3(64), 0, a);
+    mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(p.key_blocks * p.chunks), heads.y, heads.z),
+                 dim3(64 * kPromptWaves), 0, a, weights, weights_out, stride, static_cast<int>(p.chunks), part, p.keys);
+    if (p.chunks > 1)
+        mhip::launch(ctx, mx4_sum_weights_kernel, dim3(static_cast<unsigned>(mhip::ceil_div(p.keys, 256)), heads.y, heads.z), dim3(256), 0,
+                     a, part, p.keys, static_cast<int>(p.chunks), weights, weights_out, stride);
+    return mhip::check_launch("attention (4-bit, weights)");
 }
 
 template <int NB, bool FEW>
@@ -1432,31 +1433,34 @@ mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* 
         return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
     const bool keep = weights_out && a.row_tiles == 1;
     a.kept_ld = (kv_rows + 63) / 64 * 64;
-    const uint64_t part_bytes = chunks > 1 ? records * (32 * NB + 2) * sizeof(float) : 0;
+    const SumPlan sums = weights_out && !keep ? sum_plan<NB>(ctx, a, batch * a.kv_heads, kv_rows) : SumPlan{};
+    // Scratch: planes, chunk records, kept scores, chunks' sums, statistics.
+    const uint64_t record_bytes = chunks > 1 ? records * (32 * NB + 2) * sizeof(float) : 0;
     const uint64_t kept_bytes = keep ? total_rows * a.kept_ld * sizeof(float) : 0;
-    const uint64_t bytes = part_bytes + kept_bytes + (weights_out ? total_rows * 2 * sizeof(float) : 0);
+    const uint64_t bytes = sums.plane_bytes + record_bytes + kept_bytes + sums.part_bytes + (weights_out ? total_rows * 2 * sizeof(float) : 0);
+    float* part = nullptr;
     if (bytes) {
         void* ws = nullptr;
         mhip_status st = mhip::workspace(ctx, bytes, &ws);
         if (st != MHIP_OK) return st;
-        a.part_o = static_cast<float*>(ws);
+        char* at = static_cast<char*>(ws);
+        a.planes = at;
+        a.part_o = reinterpret_cast<float*>(at += sums.plane_bytes);
         a.part_ml = a.part_o + records * (32 * NB);
-        a.kept = keep ? reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part_bytes) : nullptr;
-        if (weights_out) a.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part_bytes + kept_bytes);
+        a.kept = keep ? reinterpret_cast<float*>(at + record_bytes) : nullptr;
+        part = reinterpret_cast<float*>(at += record_bytes + kept_bytes);
+        if (weights_out) a.stats = reinterpret_cast<float*>(at + sums.part_bytes);
     }
     a.arrived = ctx->mx4_arrived;
     const dim3 grid(static_cast<unsigned>(a.row_tiles * chunks), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
     mhip::launch(ctx, mx4_rows_kernel<NB, FEW>, grid, dim3(64 * kRowWaves<NB>), 0, a);
     mhip_status st = mhip::check_launch("attention (4-bit)");
     if (st != MHIP_OK || !weights_out) return st;
+    if (!keep) return launch_weights<NB>(ctx, a, batch, sums, part, weights, weights_out, stride);
     const uint64_t keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
-    const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
-    if (keep)
-        mhip::launch(ctx, mx4_kept_weights_kernel, dim3(static_cast<unsigned>(mhip::ceil_div(keys, 1024)), heads.y, heads.z),
-                     dim3(256), 0, a, weights, weights_out, stride);
-    else
-        mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(keys, 64 * kWeightWaves)), heads.y, heads.z),
-                     dim3(64 * kWeightWaves), 0, a, weights, weights_out, stride);
+    mhip::launch(ctx, mx4_kept_weights_kernel,
+                 dim3(static_cast<unsigned>(mhip::ceil_div(keys, 1024)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
+                 dim3(256), 0, a, weights, weights_out, stride);
     return mhip::check_launch("attention (4-bit, weights)");
 }
 
@@ -1466,21 +1470,13 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
     a.row_tiles = static_cast<int>(mhip::ceil_div(a.rows, kPromptRows));
     a.batch = static_cast<int>(batch);
     const uint64_t pairs = batch * a.kv_heads, tiles = pairs * a.row_tiles;
-    // The key tiles of the row tiles, all and the most.
-    uint64_t units = 0, most = 0;
-    for (int t = 0; t < a.row_tiles && t < 4096; ++t) {
-        const int i0 = t * kPromptRows / a.group, i1 = (std::min((t + 1) * kPromptRows, a.rows) - 1) / a.group;
-        const int at = a.kv - a.seq;
-        const int lo = a.window > 0 ? std::max(at + i0 - (a.window - 1), 0) : 0, hi = a.causal ? at + i1 + 1 : a.kv;
-        const uint64_t n = static_cast<uint64_t>((hi + 63) / 64 - lo / 64);
-        units += n * pairs;
-        most = std::max(most, n);
-    }
-    const uint64_t slots = 2ull * ctx->compute_units;
+    const KeyTiles keys = key_tiles(a);
+    const uint64_t units = keys.all * pairs, most = keys.most;
+    const uint64_t slots = (NB > 4 ? 1ull : 2ull) * ctx->compute_units;
     a.chunks = 1;
     a.chunk_tiles = 0;
     a.heavy_ranks = a.row_tiles;
-    if (tiles < kSplitBelow * ctx->compute_units / 4) {
+    if (tiles < ctx->compute_units) {
         const uint64_t len = std::max<uint64_t>(kMinChunk, mhip::ceil_div(units, slots));
         if (len < most) {
             a.chunk_tiles = static_cast<int>(len);
@@ -1491,30 +1487,23 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
         a.heavy_ranks = static_cast<int>(mhip::ceil_div(ctx->compute_units, pairs));
     if (tiles * a.chunks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
     const uint64_t records = a.chunks > 1 ? tiles * a.chunks * kPromptRows : 0;
-    const bool made = a.row_tiles >= kMadeFrom;
-    a.tiles_ld = mhip::ceil_div(a.kv, 64);
-    const uint64_t tile_bytes = made ? pairs * a.tiles_ld * PromptCfg<NB>::kBytes : 0;
-    a.planes_ld = static_cast<uint64_t>(a.row_tiles) * kPromptWaves;
-    const uint64_t plane_bytes = weights_out ? pairs * a.planes_ld * SumCfg<NB>::kBytes : 0;
-    const uint64_t bytes = tile_bytes + plane_bytes + records * (32 * NB + 2) * sizeof(float) + (weights_out ? pairs * a.rows * 2 * sizeof(float) : 0);
+    const SumPlan sums = weights_out ? sum_plan<NB>(ctx, a, pairs, a.kv) : SumPlan{};
+    const uint64_t record_bytes = records * (32 * NB + 2) * sizeof(float);
+    const uint64_t bytes = sums.plane_bytes + record_bytes + sums.part_bytes + (weights_out ? pairs * a.rows * 2 * sizeof(float) : 0);
+    float* part = nullptr;
     if (bytes) {
         void* ws = nullptr;
         mhip_status st = mhip::workspace(ctx, bytes, &ws);
         if (st != MHIP_OK) return st;
-        a.tiles = static_cast<char*>(ws);
-        a.planes = weights_out ? a.tiles + tile_bytes : nullptr;
-        a.part_o = reinterpret_cast<float*>(a.tiles + tile_bytes + plane_bytes);
+        char* at = static_cast<char*>(ws);
+        a.planes = at;
+        a.part_o = reinterpret_cast<float*>(at += sums.plane_bytes);
         a.part_ml = a.part_o + records * (32 * NB);
-        if (weights_out) a.stats = a.part_ml + records * 2;
+        part = reinterpret_cast<float*>(at += record_bytes);
+        if (weights_out) a.stats = reinterpret_cast<float*>(at + sums.part_bytes);
     }
     const dim3 grid(static_cast<unsigned>(tiles * a.chunks)), block(64 * kPromptWaves);
-    if (made) {
-        mhip::launch(ctx, mx4_tiles_kernel<NB>,
-                     dim3(static_cast<unsigned>(a.tiles_ld), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)), dim3(256), 0, a);
-        mhip::launch(ctx, mx4_prompt_kernel<NB, true>, grid, block, 0, a);
-    } else {
-        mhip::launch(ctx, mx4_prompt_kernel<NB, false>, grid, block, 0, a);
-    }
+    mhip::launch(ctx, mx4_prompt_kernel<NB>, grid, block, 0, a);
     mhip_status st = mhip::check_launch("attention (4-bit, prompt)");
     const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
     if (st == MHIP_OK && a.chunks > 1) {
@@ -1523,9 +1512,22 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
         st = mhip::check_launch("attention (4-bit, prompt merge)");
     }
     if (st != MHIP_OK || !weights_out) return st;
-    mhip::launch(ctx, mx4_prompt_weights_kernel<NB>, dim3(static_cast<unsigned>(mhip::ceil_div(a.kv, 32 * kPromptWaves)), heads.y, heads.z),
-                 block, 0, a, weights, weights_out, stride);
-    return mhip::check_launch("attention (4-bit, weights)");
+    return launch_weights<NB>(ctx, a, batch, sums, part, weights, weights_out, stride);
+}
+
+// Which of the two attention kernels is the faster one, in microseconds of time
+// that both were measured to take on 256 CUs (2 to 20 % off over rows of 5 to
+// 2048 queries and 1000 to 30000 keys, head dimensions 64 to 192): a workgroup
+// of the rows kernel 6, and 0.75 a block of 32 columns for each turn of its
+// waves over 64 keys; prompts 25 to fill and drain, then 0.46 a block for 128
+// rows by 64 keys on one CU. `units`: such row and key tiles in all.
+bool prompt_is_faster(const mhip_ctx* ctx, const Mx4Attn& a, uint64_t pairs, uint64_t units, uint64_t nb) {
+    const uint64_t row_tiles = mhip::ceil_div(a.rows, 16), waves = nb > 4 ? 4 : 8;
+    const double cus = ctx->compute_units, tiles = static_cast<double>(pairs * row_tiles);
+    const double chunks = std::max(1.0, std::ceil(cus / tiles));
+    const double strips = static_cast<double>(units) * std::min<double>(8, row_tiles) / tiles / chunks;  // of 64 keys a workgroup
+    const double rows_us = std::ceil(tiles * chunks / cus) * (6 + 0.75 * nb * std::ceil(strips / waves));
+    return 25 + 0.46 * nb * units / cus < rows_us;
 }
 
 }  // namespace
@@ -1610,16 +1612,19 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     }
     const uint64_t plan_rows = p->bounded_key_count ? p->kv_rows : p->kv_seq_len;
     const bool few = a.rows <= kRowTile<true>;
-    if (p->seq_len > 1 && rows >= 64) {
-        switch (mhip::mx4_blocks(d)) {
+    const uint64_t blocks = mhip::mx4_blocks(d);
+    // Above six blocks the prompts' sums do not fit the registers.
+    if (p->seq_len > 1 && rows > kRowTile<false> && blocks <= 6 && prompt_is_faster(ctx, a, batch * Hkv, key_tiles(a).all * batch * Hkv, blocks)) {
+        switch (blocks) {
             case 1: return launch_prompt<1>(ctx, a, batch, weights, weights_out, p->kv_rows);
             case 2: return launch_prompt<2>(ctx, a, batch, weights, weights_out, p->kv_rows);
             case 3: return launch_prompt<3>(ctx, a, batch, weights, weights_out, p->kv_rows);
             case 4: return launch_prompt<4>(ctx, a, batch, weights, weights_out, p->kv_rows);
-            default: break;
+            case 5: return launch_prompt<5>(ctx, a, batch, weights, weights_out, p->kv_rows);
+            default: return launch_prompt<6>(ctx, a, batch, weights, weights_out, p->kv_rows);
         }
     }
-    switch (mhip::mx4_blocks(d)) {
+    switch (blocks) {
         case 1:
             return few ? launch_rows<1, true>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows)
                        : launch_rows<1, false>(ctx, a, batch, weights, weights_out, p->kv_rows, plan_rows);

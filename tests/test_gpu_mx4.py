@@ -183,6 +183,37 @@ def test_attention_group_sizes_and_row_tiles(dev, seq, kv, heads, kv_heads):
     check_attention(dev, seq * 7 + kv + 1, seq, kv, heads, kv_heads, 64, batch=2, capacity=kv + 3)
 
 
+@pytest.mark.parametrize("seq,kv,heads,kv_heads,d,kw", [
+    # Long enough for the prompts' kernel: whole row tiles of it split over their
+    # keys, one chunk each, odd lengths, windows, blocks that are no power of two.
+    (700, 700, 32, 4, 128, {}), (513, 1500, 24, 8, 96, dict(window=333)), (1030, 1030, 16, 16, 64, {}),
+    (400, 2500, 16, 2, 80, dict(batch=2, capacity=2510)), (600, 1300, 16, 4, 32, dict(causal=False)),
+    (500, 900, 16, 4, 160, {}), (420, 1000, 16, 4, 192, dict(window=100)), (300, 700, 16, 4, 256, {}),
+    (900, 900, 32, 8, 100, dict(scale=0.3)),
+])
+def test_attention_prompts(dev, seq, kv, heads, kv_heads, d, kw):
+    check_attention(dev, seq + kv, seq, kv, heads, kv_heads, d, **kw)
+
+
+def test_attention_prompt_with_outliers_in_q(dev):
+    """Q's planes are fixed-point within a block: values 1000 times smaller than
+    their block's largest keep 2^-30 of it."""
+    from magnetar_hip import ops
+    rng = np.random.default_rng(5)
+    seq, heads, d = 600, 16, 128
+    q = rng.standard_normal((seq, heads * d)).astype(np.float32)
+    q[:, 7::32] *= 1000.0
+    k, v = cache_rows(1, seq, heads, d), cache_rows(2, seq, heads, d)
+    k[:, 7::32] *= np.float32(1e-3)
+    p = ops.attention_params(seq, seq, heads, d, causal=True)
+    out = ops.attention_mx4(dev, dev.upload(q), store_of(dev, k, seq, heads, d), store_of(dev, v, seq, heads, d), p).numpy()
+    want, _, largest = ref.attention(q, ref.round_trip(k, heads, d), ref.round_trip(v, heads, d), heads, heads, d)
+    # Each of 32 values of a block is off by at most 2^-30 of the largest, the
+    # held keys are within 6 of one another's scale: under 2^-30 * 3000 * 16 * 6 /
+    # sqrt(128) of a score, beside the sums' own.
+    assert rel(out, want) <= ref.attention_tolerance(d, largest) + 2.0 ** -30 * 3000 * 16 * 6 / np.sqrt(d)
+
+
 @pytest.mark.parametrize("causal,window", [(False, None), (True, 1), (True, 7), (True, 64), (True, 100), (True, 5000)])
 @pytest.mark.parametrize("seq,kv", [(1, 500), (9, 300), (100, 230), (300, 300)])
 def test_attention_masks(dev, causal, window, seq, kv):
@@ -224,7 +255,7 @@ def nonfinite_case(dev, seq, kv, heads, kv_heads, d, window, k_bad, v_bad, q_bad
         assert np.allclose(got[fine], expect[fine], rtol=1e-4, atol=1e-5)
 
 
-@pytest.mark.parametrize("seq,kv", [(40, 40), (40, 200), (130, 130)])
+@pytest.mark.parametrize("seq,kv", [(40, 40), (40, 200), (130, 130), (1500, 1500)])
 @pytest.mark.parametrize("window", [None, 9])
 def test_values_that_are_not_finite_reach_the_queries_that_admit_them(dev, seq, kv, window):
     """A NaN block of K or V next to the mask's edges: queries that admit the
@@ -350,7 +381,7 @@ def test_a_conversation_over_a_bounded_cache(dev):
     assert evictions >= 1
 
 
-@pytest.mark.parametrize("d,heads,kv_heads", [(64, 4, 2), (128, 8, 8), (80, 4, 1)])
+@pytest.mark.parametrize("d,heads,kv_heads", [(64, 4, 2), (128, 8, 8), (80, 4, 1), (64, 40, 1)])
 def test_a_captured_step_replays_down_the_cache(dev, d, heads, kv_heads):
     """Write, attention and account recorded once and replayed at later rows
     equal the eager calls at those rows bit for bit, eager work in between."""
