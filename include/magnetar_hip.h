@@ -556,12 +556,16 @@ mhip_kernel_error mhip_executor_write_zeroed_tensor(mhip_executor* ex, const cha
 mhip_kernel_error mhip_executor_write_weight_tensor(mhip_executor* ex, const char* id,
                                                     const uint64_t* shape, int rank,
                                                     const float* values, int* compact);
-/* KV store precisions (KvStorePrecision: F32, Tq4, Tq3). */
-typedef enum { MHIP_KV_F32 = 0, MHIP_KV_TQ4 = 1, MHIP_KV_TQ3 = 2 } mhip_kv_precision;
+/* KV store precisions (KvStorePrecision: F32, Tq4, Tq3; MX4 has no counterpart
+ * in the reference). */
+typedef enum { MHIP_KV_F32 = 0, MHIP_KV_TQ4 = 1, MHIP_KV_TQ3 = 2, MHIP_KV_MX4 = 3 } mhip_kv_precision;
 /* write_zeroed_kv_store (src/executor.rs:560-602): a zeroed f32 store of
- * `shape` under `id`, *stored = 1. The quantized TurboQuant precisions are not
- * provided by this build: *stored = 0 and nothing is written (the caller keeps
- * an f32 store). */
+ * `shape` under `id`, *stored = 1; under MHIP_KV_MX4 one that holds the same
+ * rows in 4 bits a value (mhip_mx4_store, whole heads of head_dimension), which
+ * kv-write and attention take in place of an f32 one, reads return as f32 and
+ * other Kernels refuse (DTypeUnsupported). The quantized TurboQuant precisions
+ * are not provided by this build: *stored = 0 and nothing is written (the caller
+ * keeps an f32 store). */
 mhip_kernel_error mhip_executor_write_zeroed_kv_store(mhip_executor* ex, const char* id,
                                                       const uint64_t* shape, int rank,
                                                       int precision, uint64_t head_dimension,

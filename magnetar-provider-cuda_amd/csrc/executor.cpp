@@ -98,6 +98,11 @@ struct Buffer {
     // An f32 weight stored compact as bf16 bit patterns (write_weight_tensor,
     // src/kernels.rs:1665-1723): 2 bytes per value, widened exactly on read.
     bool compact = false;
+    // A 4-bit KV store (write_zeroed_kv_store, MHIP_KV_MX4): the f32 rows that
+    // `shape` says, held as mhip_mx4_store does with heads of this dimension;
+    // 0 for any other tensor.
+    uint64_t mx4_dim = 0;
+    mhip_mx4_store mx4() const { return {shape[0], shape[1] / mx4_dim, mx4_dim, 1, 0}; }
 
     Buffer(mhip_ctx* c, size_t nbytes, Shape s, int dt) : ctx(c), bytes(nbytes), shape(std::move(s)), dtype(dt) {
         check(mhip_alloc(ctx, bytes, &ptr));
@@ -286,7 +291,7 @@ struct mhip_executor {
     // (`alloc_output`, src/kernels.rs:2342-2355), else a fresh one.
     BufferPtr alloc_output(BufferPtr& offered, const Shape& shape, int dtype) {
         const size_t bytes = numel(shape) * dtype_size(dtype);
-        if (offered && offered->bytes == bytes && !offered->compact) {
+        if (offered && offered->bytes == bytes && !offered->compact && !offered->mx4_dim) {
             BufferPtr out = std::move(offered);
             out->shape = shape;
             out->dtype = dtype;
@@ -299,6 +304,8 @@ struct mhip_executor {
         if (b.dtype != MHIP_DTYPE_F32)
             raise(MHIP_KERNEL_DTYPE_UNSUPPORTED,
                   std::string(what) + " reads f32 operands, got " + dtype_name(b.dtype));
+        if (b.mx4_dim)
+            raise(MHIP_KERNEL_DTYPE_UNSUPPORTED, std::string(what) + " does not read 4-bit KV stores");
     }
 
     static std::pair<uint64_t, uint64_t> rows_cols(const Buffer& b) {
@@ -697,10 +704,17 @@ struct mhip_executor {
                 raise(MHIP_KERNEL_ATTRIBUTE_UNSUPPORTED,
                       std::string("attention ") + unsupported + " is not implemented by this Provider");
         require_f32(q, "attention");
-        require_f32(k, "attention");
-        require_f32(v, "attention");
         const uint64_t H = *head_count, d = *head_dim;
         const uint64_t vd = value_dim.value_or(d);
+        const bool mx4 = k.mx4_dim || v.mx4_dim;
+        if (mx4 && !(k.mx4_dim == d && v.mx4_dim == d && vd == d))
+            raise(MHIP_KERNEL_LAYOUT_UNSUPPORTED,
+                  "attention over 4-bit KV stores takes two of head dimension " + std::to_string(d) + ", got " +
+                      std::to_string(k.mx4_dim) + " and " + std::to_string(v.mx4_dim));
+        if (!mx4) {
+            require_f32(k, "attention");
+            require_f32(v, "attention");
+        }
         if (vd == d && k.shape != v.shape)
             raise(MHIP_KERNEL_SHAPE_UNSUPPORTED,
                   "shape mismatch: " + fmt_shape(k.shape) + " vs " + fmt_shape(v.shape));
@@ -759,7 +773,8 @@ struct mhip_executor {
         p.batch = 1;
         p.bounded_key_count = key_count.has_value() ? 1 : 0;
         BufferPtr out = alloc_output(offered, Shape{seq, H * vd}, MHIP_DTYPE_F32);
-        check(mhip_attention_f32(ctx, q.f(), k.f(), v.f(), out->f(), &p));
+        check(mx4 ? mhip_attention_mx4(ctx, q.f(), k.ptr, v.ptr, out->f(), &p, nullptr, nullptr)
+                  : mhip_attention_f32(ctx, q.f(), k.f(), v.f(), out->f(), &p));
         return out;
     }
 
@@ -804,6 +819,7 @@ struct mhip_executor {
         std::unique_ptr<Buffer> ta, tb;
         auto as_half = [&](const Buffer& x, std::unique_ptr<Buffer>& tmp) -> const uint16_t* {
             if (x.dtype == dtype) return x.h();
+            if (x.mx4_dim) raise(MHIP_KERNEL_DTYPE_UNSUPPORTED, "a half-precision operand is a 4-bit KV store");
             if (x.dtype != MHIP_DTYPE_F32)
                 raise(MHIP_KERNEL_DTYPE_UNSUPPORTED,
                       std::string("operand stored as ") + dtype_name(x.dtype) + ", expected " + dtype_name(dtype));
@@ -856,6 +872,7 @@ struct mhip_executor {
     BufferPtr clone(const Buffer& b) {
         BufferPtr copy = std::make_unique<Buffer>(ctx, b.bytes, b.shape, b.dtype);
         copy->compact = b.compact;
+        copy->mx4_dim = b.mx4_dim;
         check(mhip_copy(ctx, copy->ptr, b.ptr, b.bytes));
         return copy;
     }
@@ -891,7 +908,7 @@ struct mhip_executor {
             if (rit == storage.end())
                 raise(MHIP_KERNEL_EXECUTION_FAILED, "no materialized data for input resource " + rows_id);
             const Buffer& rows = *rit->second;
-            require_f32(*store, "kv-write");
+            if (!store->mx4_dim) require_f32(*store, "kv-write");
             require_f32(rows, "kv-write");
             const auto [capacity, width] = rows_cols(*store);
             const auto [count, row_width] = rows_cols(rows);
@@ -899,7 +916,12 @@ struct mhip_executor {
                 raise(MHIP_KERNEL_SHAPE_UNSUPPORTED, "kv-write rows have width " +
                                                          std::to_string(row_width) + ", the store " +
                                                          std::to_string(width));
-            check(mhip_kv_write_f32(ctx, store->f(), capacity, width, rows.f(), count, *row_offset));
+            if (store->mx4_dim) {
+                const mhip_mx4_store shape = store->mx4();
+                check(mhip_kv_write_mx4(ctx, store->ptr, &shape, rows.f(), count, *row_offset));
+            } else {
+                check(mhip_kv_write_f32(ctx, store->f(), capacity, width, rows.f(), count, *row_offset));
+            }
         } catch (const KernelFailure& f) {
             code = f.code;
             error = f.detail;
@@ -1163,14 +1185,22 @@ mhip_kernel_error mhip_executor_write_zeroed_kv_store(mhip_executor* ex, const c
                                                       const uint64_t* shape, int rank,
                                                       int precision, uint64_t head_dimension,
                                                       int* stored) {
-    (void)head_dimension;  // used by the quantized stores only
     return guarded([&] {
         if (!ex || !id) raise(MHIP_KERNEL_EXECUTION_FAILED, "null executor or id");
         if (stored) *stored = 0;
-        if (precision != MHIP_KV_F32) return;
+        if (precision != MHIP_KV_F32 && precision != MHIP_KV_MX4) return;
         Shape s = make_shape(shape, rank);
+        size_t bytes = numel(s) * 4;
+        if (precision == MHIP_KV_MX4) {
+            if (s.size() != 2 || head_dimension == 0 || s[1] == 0 || s[1] % head_dimension != 0)
+                raise(MHIP_KERNEL_SHAPE_UNSUPPORTED, "a 4-bit KV store holds rows of whole heads of " +
+                                                         std::to_string(head_dimension) + ", got shape " + fmt_shape(s));
+            bytes = mhip_kv_mx4_bytes(s[0], s[1] / head_dimension, head_dimension);
+            if (bytes == 0 && s[0] != 0) raise(MHIP_KERNEL_SHAPE_UNSUPPORTED, mhip_last_error_detail());
+        }
         std::lock_guard<std::mutex> lock(ex->mu);
-        auto buf = std::make_unique<Buffer>(ex->ctx, numel(s) * 4, s, MHIP_DTYPE_F32);
+        auto buf = std::make_unique<Buffer>(ex->ctx, bytes, s, MHIP_DTYPE_F32);
+        if (precision == MHIP_KV_MX4) buf->mx4_dim = head_dimension;
         check(mhip_zero(ex->ctx, buf->ptr, buf->bytes));
         ex->storage[id] = std::move(buf);
         if (stored) *stored = 1;
@@ -1188,6 +1218,16 @@ void download_widened(mhip_ctx* ctx, const Buffer& b, uint64_t first, uint64_t c
         const uint32_t u = static_cast<uint32_t>(bits[i]) << 16;
         std::memcpy(dst + i, &u, 4);
     }
+}
+
+// The values of rows [begin, begin + count) of a 4-bit KV store, on the host.
+void download_rows(mhip_ctx* ctx, const Buffer& b, uint64_t begin, uint64_t count, float* dst) {
+    const uint64_t width = b.shape[1];
+    if (count == 0) return;
+    Buffer rows(ctx, count * width * 4, Shape{count, width}, MHIP_DTYPE_F32);
+    const mhip_mx4_store shape = b.mx4();
+    check(mhip_kv_read_mx4(ctx, b.ptr, &shape, rows.f(), count, begin));
+    check(mhip_download(ctx, dst, rows.ptr, rows.bytes));
 }
 
 }  // namespace
@@ -1245,12 +1285,15 @@ mhip_kernel_error mhip_executor_read_tensor(mhip_executor* ex, const char* id, v
         if (it == ex->storage.end())
             raise(MHIP_KERNEL_EXECUTION_FAILED, std::string("no materialized data for resource ") + id);
         const Buffer& b = *it->second;
-        if (b.compact) {
+        if (b.compact || b.mx4_dim) {
             const uint64_t n = numel(b.shape);
             if (capacity < n * 4)
                 raise(MHIP_KERNEL_SHAPE_UNSUPPORTED, "destination holds " + std::to_string(capacity) +
                                                          " bytes, tensor has " + std::to_string(n * 4));
-            download_widened(ex->ctx, b, 0, n, static_cast<float*>(dst));
+            if (b.compact)
+                download_widened(ex->ctx, b, 0, n, static_cast<float*>(dst));
+            else
+                download_rows(ex->ctx, b, 0, b.shape[0], static_cast<float*>(dst));
             if (written) *written = n * 4;
             return;
         }
@@ -1278,6 +1321,8 @@ mhip_kernel_error mhip_executor_read_tensor_values(mhip_executor* ex, const char
                                                      " values, tensor has " + std::to_string(n));
         if (b.compact) {
             download_widened(ex->ctx, b, 0, n, dst);
+        } else if (b.mx4_dim) {
+            download_rows(ex->ctx, b, 0, b.shape[0], dst);
         } else if (b.dtype == MHIP_DTYPE_F32) {
             check(mhip_download(ex->ctx, dst, b.ptr, n * 4));
         } else {
@@ -1311,6 +1356,8 @@ mhip_kernel_error mhip_executor_read_tensor_rows(mhip_executor* ex, const char* 
         if (capacity < row_count * width) raise(MHIP_KERNEL_SHAPE_UNSUPPORTED, "destination too small");
         if (b.compact)
             download_widened(ex->ctx, b, row_begin * width, row_count * width, dst);
+        else if (b.mx4_dim)
+            download_rows(ex->ctx, b, row_begin, row_count, dst);
         else
             check(mhip_download(ex->ctx, dst, b.f() + row_begin * width, row_count * width * 4));
     });
@@ -1354,6 +1401,7 @@ mhip_kernel_error mhip_executor_copy_tensor(mhip_executor* ex, const char* src, 
         const Buffer& b = *it->second;
         auto copy = std::make_unique<Buffer>(ex->ctx, b.bytes, b.shape, b.dtype);
         copy->compact = b.compact;
+        copy->mx4_dim = b.mx4_dim;
         check(mhip_copy(ex->ctx, copy->ptr, b.ptr, b.bytes));
         ex->storage[dst] = std::move(copy);
     });
@@ -1562,7 +1610,7 @@ mhip_kernel_error mhip_executor_replay_step(mhip_executor* ex, const char* id, u
         }
         for (int i = 0; i < input_count; ++i) {
             Buffer& buffer = *ex->storage[input_ids[i]];
-            if (buffer.dtype != MHIP_DTYPE_F32 || input_lengths[i] * 4 != buffer.bytes)
+            if (buffer.dtype != MHIP_DTYPE_F32 || buffer.mx4_dim || input_lengths[i] * 4 != buffer.bytes)
                 raise(MHIP_KERNEL_EXECUTION_FAILED,
                       std::string("replay input '") + input_ids[i] + "' has " +
                           std::to_string(input_lengths[i]) + " values, its buffer " +

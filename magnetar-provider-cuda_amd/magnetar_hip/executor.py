@@ -16,8 +16,9 @@ import numpy as np
 from . import _lib
 
 F32, F16, BF16 = 0, 1, 2
-# KV store precisions (KvStorePrecision); only KV_F32 stores are provided.
-KV_F32, KV_TQ4, KV_TQ3 = 0, 1, 2
+# KV store precisions (KvStorePrecision, and the 4-bit KV_MX4); KV_F32 and
+# KV_MX4 stores are provided.
+KV_F32, KV_TQ4, KV_TQ3, KV_MX4 = 0, 1, 2, 3
 DTYPE_NAMES = {F32: "Float32", F16: "Float16", BF16: "BrainFloat16"}
 
 KERNEL_ERRORS = {
@@ -300,8 +301,9 @@ class Executor:
 
     def write_zeroed_kv_store(self, id: str, shape: Sequence[int], precision: int = KV_F32,
                               head_dimension: int = 0) -> bool:
-        """A zeroed KV store (src/executor.rs:560-602). True when stored; the
-        quantized precisions are declined (False) and nothing is written."""
+        """A zeroed KV store (src/executor.rs:560-602), of f32 values or (KV_MX4,
+        heads of `head_dimension`) in 4 bits a value. True when stored; the
+        other precisions are declined (False) and nothing is written."""
         shp, rank = _shape(shape)
         stored = ctypes.c_int(0)
         _check(_lib_bound().mhip_executor_write_zeroed_kv_store(
