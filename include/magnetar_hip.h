@@ -375,8 +375,9 @@ mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, const void* v_
  * transfers, clears memory or synchronises can be captured: such a call
  * returns CaptureUnsupported and fails the capture (mhip_capture_end then
  * reports the first reason). Growing the workspace is such an allocation, but
- * for products and prompt attention that could run without that scratch: for
- * them it grows while recording, so that a capture takes the eager call's plan. Multi-row attention replays only at offset 0. */
+ * for products and prompt attention that could run without that scratch and for
+ * 4-bit stores: for them it grows while recording, so that a capture takes the
+ * eager call's plan. Multi-row attention replays only at offset 0. */
 typedef enum {
     MHIP_ADVANCE_POSITION_OFFSET = 1,
     MHIP_ADVANCE_KEY_COUNT = 2,

@@ -1405,7 +1405,7 @@ template <int NB>
 mhip_status launch_weights(mhip_ctx* ctx, const Mx4Attn& a, uint64_t batch, const SumPlan& p, float* part, const float* weights,
                            float* weights_out, uint64_t stride) {
     const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
-    if (p.key_blocks * p.chunks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    if (p.key_blocks * p.chunks * kPromptWaves * 64 >= (1ULL << 32)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
     mhip::launch(ctx, mx4_planes_kernel<NB>, dim3(static_cast<unsigned>(a.planes_ld), heads.y, heads.z), dim3(64), 0, a);
     mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(p.key_blocks * p.chunks), heads.y, heads.z),
                  dim3(64 * kPromptWaves), 0, a, weights, weights_out, stride, static_cast<int>(p.chunks), part, p.keys);
@@ -1429,7 +1429,7 @@ mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* 
     a.chunks = static_cast<int>(chunks);
     const uint64_t records = tiles * chunks * kRowTile<FEW>;
     const uint64_t total_rows = batch * a.kv_heads * static_cast<uint64_t>(a.rows);
-    if (a.row_tiles * chunks >= (1ULL << 31) || mhip::ceil_div(total_rows, 4) >= (1ULL << 31))
+    if (a.row_tiles * chunks * kRowWaves<NB> * 64 >= (1ULL << 32))
         return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
     const bool keep = weights_out && a.row_tiles == 1;
     a.kept_ld = (kv_rows + 63) / 64 * 64;
@@ -1485,7 +1485,7 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
     }
     if (a.chunks == 1 && tiles > ctx->compute_units && tiles <= slots)
         a.heavy_ranks = static_cast<int>(mhip::ceil_div(ctx->compute_units, pairs));
-    if (tiles * a.chunks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    if (tiles * a.chunks * kPromptWaves * 64 >= (1ULL << 32)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
     const uint64_t records = a.chunks > 1 ? tiles * a.chunks * kPromptRows : 0;
     const SumPlan sums = weights_out ? sum_plan<NB>(ctx, a, pairs, a.kv) : SumPlan{};
     const uint64_t record_bytes = records * (32 * NB + 2) * sizeof(float);
@@ -1575,7 +1575,8 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     if (!mhip::aligned16(k_store) || !mhip::aligned16(v_store))
         return mhip::fail(MHIP_LAYOUT_UNSUPPORTED, "attention: the stores must be 16-byte aligned");
     const uint64_t group = H / Hkv, rows = p->seq_len * group;
-    if (H >= (1ULL << 20) || rows >= (1ULL << 31) - 512)
+    // A grid has fewer than 2^32 threads.
+    if (H >= (1ULL << 20) || rows >= (1ULL << 26))
         return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
 
     Mx4Attn a{};
@@ -1613,6 +1614,7 @@ extern "C" mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const v
     const uint64_t plan_rows = p->bounded_key_count ? p->kv_rows : p->kv_seq_len;
     const bool few = a.rows <= kRowTile<true>;
     const uint64_t blocks = mhip::mx4_blocks(d);
+    const mhip::CaptureGrowth growth(ctx, true);  // a capture takes the eager call's plan
     // Above six blocks the prompts' sums do not fit the registers.
     if (p->seq_len > 1 && rows > kRowTile<false> && blocks <= 6 && prompt_is_faster(ctx, a, batch * Hkv, key_tiles(a).all * batch * Hkv, blocks)) {
         switch (blocks) {

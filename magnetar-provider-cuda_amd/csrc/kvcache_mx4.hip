@@ -328,6 +328,28 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
     for (uint32_t j = a.keep + tid; j < a.out_rows; j += kSelectThreads) a.weights_out[blockIdx.x * a.out_stride + j] = 0.0f;
 }
 
+// The NB bytes of row r of a unit (`from`, as aligned as NB's power of two)
+// into the unit's dwords.
+template <int NB>
+__device__ __forceinline__ void take_row(const uint8_t* from, int r, uint32_t (&code)[NB]) {
+    if constexpr (NB % 4 == 0) {
+#pragma unroll
+        for (int w = 0; w < NB / 4; ++w) code[r * (NB / 4) + w] = reinterpret_cast<const uint32_t*>(from)[w];
+    } else if constexpr (NB % 2 == 0) {
+#pragma unroll
+        for (int w = 0; w < NB / 2; ++w) {
+            const int at = r * (NB / 2) + w;  // half dword of the unit
+            code[at / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[w]) << (16 * (at % 2));
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < NB; ++p) {
+            const int at = r * NB + p;
+            code[at / 4] |= static_cast<uint32_t>(from[p]) << (8 * (at % 4));
+        }
+    }
+}
+
 // Rows of `src` to rows 0 .. keep - 1 of `dst`: row indices[i], or i itself
 // where indices is null. 16 lanes a group of four rows, as for a write;
 // blockIdx.y: the keys' or the values' store.
@@ -355,12 +377,7 @@ __global__ __launch_bounds__(256) void mx4_move_kernel(MoveArgs a) {
     for (int r = 0; r < 4; ++r) {
         if (r >= hi) continue;
         const uint32_t row = a.indices ? a.indices[bh * a.keep + group * 4 + r] : group * 4 + r;
-        const uint8_t* from = unit_ptr<NB>(src, b, h, row / 4, n) + (row % 4) * NB;
-#pragma unroll
-        for (int p = 0; p < NB; ++p) {
-            const int at = r * NB + p;
-            code[at / 4] |= static_cast<uint32_t>(from[p]) << (8 * (at % 4));
-        }
+        take_row<NB>(unit_ptr<NB>(src, b, h, row / 4, n) + (row % 4) * NB, r, code);
         if (n < NB) scale |= static_cast<uint32_t>(scale_ptr<NB>(src, b, h, row / 4)[4 * n + row % 4]) << (8 * r);
     }
     uint8_t* to = unit_ptr<NB>(dst, b, h, group, n);
@@ -386,7 +403,7 @@ mhip_status move_rows(mhip_ctx* ctx, MoveArgs& a, uint64_t batch, uint64_t heads
     a.groups_touched = static_cast<uint32_t>(mhip::ceil_div(a.keep, 4));
     a.units = batch * heads * a.groups_touched;
     const uint64_t blocks = mhip::ceil_div(a.units, 16);
-    if (blocks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-evict: too many rows");
+    if (blocks >= (1ULL << 24)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-evict: too many rows");
     const dim3 grid(static_cast<unsigned>(blocks), 2);
     switch (nb) {
         case 1: mhip::launch(ctx, mx4_move_kernel<1>, grid, dim3(256), 0, a); break;
@@ -445,7 +462,8 @@ extern "C" mhip_status mhip_kv_write_mx4(mhip_ctx* ctx, void* store, const mhip_
     const uint64_t batch = shape->batch ? shape->batch : 1, nb = mhip::mx4_blocks(shape->head_dimension);
     const uint64_t touched = advance ? mhip::ceil_div(count + 3, 4) : (row_offset + count - 1) / 4 - row_offset / 4 + 1;
     const uint64_t units = batch * touched * shape->kv_heads, blocks = mhip::ceil_div(units, 16);
-    if (blocks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-write: too many rows");
+    // A grid has fewer than 2^32 threads.
+    if (blocks >= (1ULL << 24)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-write: too many rows");
     const StoreArgs s = store_args(*shape, store);
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
     const uint32_t t = static_cast<uint32_t>(touched);
@@ -472,7 +490,7 @@ extern "C" mhip_status mhip_kv_read_mx4(mhip_ctx* ctx, const void* store, const 
     const uint64_t batch = shape->batch ? shape->batch : 1, nb = mhip::mx4_blocks(shape->head_dimension);
     const uint64_t touched = (row_offset + count - 1) / 4 - row_offset / 4 + 1;
     const uint64_t units = batch * touched * shape->kv_heads, blocks = mhip::ceil_div(units, 16);
-    if (blocks >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-read: too many rows");
+    if (blocks >= (1ULL << 24)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-read: too many rows");
     const StoreArgs s = store_args(*shape, store);
     const dim3 grid(static_cast<unsigned>(blocks)), block(256);
     const uint32_t t = static_cast<uint32_t>(touched);
@@ -536,7 +554,7 @@ extern "C" mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, con
         return mhip::fail(MHIP_LAYOUT_UNSUPPORTED,
                           "kv-evict: the output stores overlap the stores (in place: the same stores and shape)");
     const uint64_t rows = batch * heads;
-    if (rows >= (1ULL << 31)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-evict: too many heads");
+    if (rows >= (1ULL << 22)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "kv-evict: too many heads");
     const uint64_t w_bytes = (rows - 1) * w_stride * 4 + p->key_count * 4;
     const uint64_t o_bytes = (rows - 1) * o_stride * 4 + out_shape->capacity * 4;
     if (!(weights_out == weights && w_stride == o_stride) && overlap(weights, w_bytes, weights_out, o_bytes))
@@ -548,6 +566,7 @@ extern "C" mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, con
     const uint64_t one = mhip::mx4_bytes(p->keep, heads, d);
     const uint64_t bytes = index_bytes + (in_place ? 2 * batch * one : 0);
     uint8_t* scratch = nullptr;
+    const mhip::CaptureGrowth growth(ctx, true);
     if (bytes) {
         void* ws = nullptr;
         st = mhip::workspace(ctx, bytes, &ws);

@@ -7,6 +7,7 @@ the way `CudaDeviceBuffer` carries its shape (reference src/kernels.rs:253-379).
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Sequence
 
 import numpy as np
@@ -38,7 +39,7 @@ class DeviceArray:
 
     @property
     def size(self) -> int:
-        return int(np.prod(self.shape, dtype=np.int64))
+        return math.prod(self.shape)
 
     def free(self) -> None:
         if self._owned and self.ptr:

@@ -191,11 +191,14 @@ class Mx4Store:
     """A 4-bit KV store (mhip_mx4_store): the f32 rows [capacity, kv_heads *
     head_dimension] of `batch` sequences, zeroed, or in `data`."""
 
-    __slots__ = ("data", "shape")
+    __slots__ = ("data", "shape", "width", "batch", "_ref", "_key")
 
     def __init__(self, dev: Device, capacity: int, kv_heads: int, head_dimension: int,
                  batch: int = 1, data: DeviceArray | None = None):
         self.shape = _lib.Mx4StoreShape(capacity, kv_heads, head_dimension, batch, 0)
+        self.width, self.batch = kv_heads * head_dimension, batch
+        self._ref = ctypes.byref(self.shape)
+        self._key = (capacity, kv_heads, head_dimension, batch)
         nbytes = _lib.lib().mhip_kv_mx4_bytes(capacity, kv_heads, head_dimension) * batch
         if nbytes == 0 and capacity:
             raise ValueError("unsupported 4-bit store shape")
@@ -205,31 +208,24 @@ class Mx4Store:
             raise ValueError(f"a store of {nbytes} bytes in a buffer of {data.nbytes}")
         self.data = data
 
-    @property
-    def width(self) -> int:
-        return self.shape.kv_heads * self.shape.head_dimension
-
 
 def kv_write_mx4(dev: Device, store: Mx4Store, rows: DeviceArray, row_offset: int) -> Mx4Store:
     """Rows [row_offset, row_offset + count) of each sequence's store = rows
     [batch, count, width], in place."""
-    per = store.shape.batch * store.width
-    count = rows.size // per
-    if rows.size != count * per:
+    count, rest = divmod(rows.size, store.batch * store.width)
+    if rest:
         raise ValueError("kv-write rows must be [batch, count, store width]")
-    call("mhip_kv_write_mx4", dev.ctx, _p(store.data), ctypes.byref(store.shape), _p(rows), count,
-         row_offset)
+    call("mhip_kv_write_mx4", dev.ctx, _p(store.data), store._ref, _p(rows), count, row_offset)
     return store
 
 
 def kv_read_mx4(dev: Device, store: Mx4Store, row_offset: int, count: int, out=None) -> DeviceArray:
     """The f32 values that rows [row_offset, row_offset + count) hold."""
-    shape = (store.shape.batch, count, store.width)
-    if out is not None and out.size != shape[0] * count * shape[2]:
+    if out is None:
+        out = dev.empty((store.batch, count, store.width))
+    elif out.size != store.batch * count * store.width:
         raise ValueError("kv-read out must be [batch, count, store width]")
-    out = _out(dev, out, shape)
-    call("mhip_kv_read_mx4", dev.ctx, _p(store.data), ctypes.byref(store.shape), _p(out), count,
-         row_offset)
+    call("mhip_kv_read_mx4", dev.ctx, _p(store.data), store._ref, _p(out), count, row_offset)
     return out
 
 
@@ -238,16 +234,14 @@ def attention_mx4(dev: Device, q: DeviceArray, k: Mx4Store, v: Mx4Store,
                   weights_out: DeviceArray | None = None) -> DeviceArray:
     """attention over 4-bit stores; weights_out = weights (or zeros) + the
     attention each key received, [batch, kv_heads, kv_rows]."""
-    for store in (k, v):
-        s = store.shape
-        if (s.capacity, s.kv_heads, s.head_dimension, s.batch) != (
-                params.kv_rows, params.kv_head_count, params.head_dimension, max(1, params.batch)):
-            raise ValueError("attention parameters differ from the store's shape")
+    key = (params.kv_rows, params.kv_head_count, params.head_dimension, params.batch or 1)
+    if k._key != key or v._key != key:
+        raise ValueError("attention parameters differ from the store's shape")
     for w in (weights, weights_out):
-        if w is not None and w.size != k.shape.batch * k.shape.kv_heads * k.shape.capacity:
+        if w is not None and w.size != key[0] * key[1] * key[3]:
             raise ValueError("attention weights must be [batch, kv_heads, kv_rows]")
-    out = _out(dev, out, (params.seq_len * max(1, params.batch),
-                          params.head_count * params.head_dimension))
+    if out is None:
+        out = dev.empty((params.seq_len * key[3], params.head_count * params.head_dimension))
     call("mhip_attention_mx4", dev.ctx, _p(q), _p(k.data), _p(v.data), _p(out),
          ctypes.byref(params), _p(weights), _p(weights_out))
     return out
@@ -259,18 +253,16 @@ def kv_evict_mx4(dev: Device, k: Mx4Store, v: Mx4Store, weights: DeviceArray, ke
     """Keeps `keep` of the key_count rows of each head: the `first` first, the
     `recent` last and those of the largest weights between. The output stores
     and weights may be the inputs themselves."""
-    heads = k.shape.batch * k.shape.kv_heads
+    heads = k._key[1] * k._key[3]
     if weights.size != heads * weights.shape[-1] or weights_out.size != heads * weights_out.shape[-1]:
         raise ValueError("kv-evict weights must be [batch, kv_heads, rows]")
     if indices is not None and indices.size != heads * keep:
         raise ValueError("kv-evict indices must be [batch, kv_heads, keep]")
-    for store in (v, k_out, v_out):
-        if bytes(store.shape) != bytes((k if store is v else k_out).shape):
-            raise ValueError("kv-evict: the key and the value store differ in shape")
+    if k._key != v._key or k_out._key != v_out._key:
+        raise ValueError("kv-evict: the key and the value store differ in shape")
     p = _lib.KvEvictParams(key_count, keep, first, recent, weights.shape[-1], weights_out.shape[-1])
-    call("mhip_kv_evict_mx4", dev.ctx, _p(k.data), _p(v.data), _p(weights), ctypes.byref(k.shape),
-         ctypes.byref(p), _p(k_out.data), _p(v_out.data), ctypes.byref(k_out.shape), _p(weights_out),
-         _p(indices))
+    call("mhip_kv_evict_mx4", dev.ctx, _p(k.data), _p(v.data), _p(weights), k._ref,
+         ctypes.byref(p), _p(k_out.data), _p(v_out.data), k_out._ref, _p(weights_out), _p(indices))
 
 
 def greedy_select(dev: Device, logits: DeviceArray, row: int = 0, excluded=(),

@@ -445,3 +445,94 @@ def test_a_captured_eviction_replays(dev):
             assert np.array_equal(got[0, h], ref.evict(weights[0, h], 190, 50, 1, 9))
         dev.zeros((64,)).numpy()
     captured.close()
+
+
+def test_a_fresh_context_captures_all_calls():
+    """A context without scratch records the calls that need some and replays
+    them with the eager call's bits; two captures share the scratch."""
+    import magnetar_hip
+    from magnetar_hip import ops
+    heads, kv_heads, d, kv, seq = 8, 2, 64, 900, 70
+    rng = np.random.default_rng(9)
+    rows = {n: cache_rows(i, kv, kv_heads, d) for i, n in enumerate("kv")}
+    q_host = rng.standard_normal((seq, heads * d)).astype(np.float32)
+
+    def calls(dev, st):
+        p = ops.attention_params(seq, kv, heads, d, kv_head_count=kv_heads, causal=True)
+        ops.attention_mx4(dev, st["q"], st["k"], st["v"], p, out=st["o"], weights_out=st["w"])
+        ops.kv_evict_mx4(dev, st["k"], st["v"], st["w"], kv, 300, st["k2"], st["v2"], st["w2"], first=2, recent=50)
+        p1 = ops.attention_params(1, 300, heads, d, kv_head_count=kv_heads)
+        ops.attention_mx4(dev, st["q1"], st["k2"], st["v2"], p1, out=st["o1"], weights=st["w2"], weights_out=st["w3"])
+
+    def state(dev):
+        st = {n: ops.Mx4Store(dev, kv, kv_heads, d) for n in "kv"}
+        for n in "kv":
+            ops.kv_write_mx4(dev, st[n], dev.upload(rows[n]), 0)
+        st |= {n: ops.Mx4Store(dev, 300, kv_heads, d) for n in ("k2", "v2")}
+        st |= {"q": dev.upload(q_host), "q1": dev.upload(q_host[:1]), "o": dev.zeros((seq, heads * d)),
+               "o1": dev.zeros((1, heads * d)), "w": dev.zeros((1, kv_heads, kv)),
+               "w2": dev.zeros((1, kv_heads, 300)), "w3": dev.zeros((1, kv_heads, 300))}
+        return st
+
+    with magnetar_hip.Device(0) as eager:
+        st = state(eager)
+        calls(eager, st)
+        want = {n: st[n].numpy() for n in ("o", "w", "w2", "o1", "w3")}
+        del st
+    with magnetar_hip.Device(0) as dev:
+        st = state(dev)
+        graphs = []
+        for _ in range(2):
+            dev.capture_begin()
+            calls(dev, st)
+            graphs.append(dev.capture_end())
+        for turn in range(4):
+            for n in ("o", "o1", "w3"):
+                dev.write(st[n], np.zeros(st[n].shape, np.float32))
+            graphs[turn % 2].launch()
+            dev.sync()
+            for n, x in want.items():
+                assert_bitexact(st[n].numpy(), x, f"{n}, replay {turn}")
+        for g in graphs:
+            g.close()
+        del st
+
+
+def test_two_contexts_side_by_side(dev):
+    """The chunks' counters and the scratch are a context's own."""
+    import magnetar_hip
+    from magnetar_hip import ops
+    heads, d, kv = 4, 128, 6000
+    rows = [cache_rows(i, kv, heads, d) for i in range(2)]
+    q = np.random.default_rng(2).standard_normal((1, heads * d)).astype(np.float32)
+    with magnetar_hip.Device(0) as other:
+        sides = []
+        for side in (dev, other):
+            sides.append((side, side.upload(q), store_of(side, rows[0], kv, heads, d), store_of(side, rows[1], kv, heads, d),
+                          ops.attention_params(1, kv, heads, d), [side.zeros((1, heads * d)) for _ in range(20)]))
+        for i in range(20):
+            for side, x, k, v, p, outs in sides:
+                ops.attention_mx4(side, x, k, v, p, out=outs[i])
+        first = sides[0][5][0].numpy()
+        for side in sides:
+            for o in side[5]:
+                assert_bitexact(o.numpy(), first)
+        del side, sides, o, outs, x, k, v
+
+
+def test_unaligned_rows_and_outputs(dev):
+    """Queries and outputs at 4-byte addresses take the scalar forms."""
+    from magnetar_hip import DeviceArray, ops
+    heads, d = 4, 64
+    for seq, kv in ((1, 300), (40, 300), (700, 1200)):
+        k, v = (store_of(dev, cache_rows(i, kv, heads, d), kv, heads, d) for i in range(2))
+        q = np.random.default_rng(seq).standard_normal((seq, heads * d)).astype(np.float32)
+        p = ops.attention_params(seq, kv, heads, d, causal=True)
+        want = ops.attention_mx4(dev, dev.upload(q), k, v, p).numpy()
+        held = dev.upload(np.concatenate([[0.0], q.ravel()]).astype(np.float32))
+        into = dev.zeros((seq * heads * d + 1,))
+        ops.attention_mx4(dev, DeviceArray(dev, held.ptr + 4, q.shape, np.float32, owned=False), k, v, p,
+                          out=DeviceArray(dev, into.ptr + 4, q.shape, np.float32, owned=False))
+        got = into.numpy()
+        assert got[0] == 0.0
+        assert_bitexact(got[1:].reshape(q.shape), want)
