@@ -1394,9 +1394,9 @@ SumPlan sum_plan(mhip_ctx* ctx, Mx4Attn& a, uint64_t pairs, uint64_t kv_rows) {
     p.keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
     const uint64_t row_blocks = mhip::ceil_div(a.rows, 32);
     a.planes_ld = row_blocks;
-    // Four workgroups for each CU, of at least eight row tiles.
+    // Two workgroups for each CU, of at least eight row tiles.
     p.key_blocks = mhip::ceil_div(p.keys, kSumKeys);
-    p.chunks = std::max<uint64_t>(1, std::min(mhip::ceil_div(4ull * ctx->compute_units, p.key_blocks * pairs), row_blocks / kSumRows));
+    p.chunks = std::max<uint64_t>(1, std::min(mhip::ceil_div(2ull * ctx->compute_units, p.key_blocks * pairs), row_blocks / kSumRows));
     p.plane_bytes = pairs * row_blocks * SumCfg<NB>::kBytes;
     p.part_bytes = p.chunks > 1 ? (pairs * p.chunks * p.keys * sizeof(float) + 15) / 16 * 16 : 0;
     return p;

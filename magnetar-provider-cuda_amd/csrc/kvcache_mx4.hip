@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(float* __restrict__ rows,
 // Eviction
 // ---------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024, kSelectPer = 8;
+constexpr int kSelectThreads = 1024;
 
 struct SelectArgs {
     const float* weights;  // [batch * heads][weight_stride]
@@ -197,13 +197,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // for itself, so that a byte costs one barrier. Then, in one scan, the rows
 // above the threshold and the first ones at it, in order.
 //
-// A thread has kPer rows side by side. Up to kPer * 1024 rows their keys stay
-// in its registers over the five passes (CACHED); longer accounts are read
-// again, stretch by stretch. What it waits for is latency: a pass of 8192
-// weights is 4 loads a thread.
-template <bool CACHED>
+// A thread has kPer rows side by side. Up to 16 * 1024 rows (CACHED) their keys
+// stay in its registers over the five passes, 8 or 16 a thread; longer accounts
+// are read again, stretch by stretch. What it waits for is latency: 8 x 8
+// accounts of 8192 weights 15 us, 2 MB.
+template <int kPer, bool CACHED>
 __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a) {
-    constexpr int kPer = kSelectPer;
     constexpr uint32_t kStretch = kPer * kSelectThreads;
     __shared__ uint32_t hist[4][256];
     __shared__ uint32_t wave_above[kSelectThreads / 64], wave_equal[kSelectThreads / 64];
@@ -211,16 +210,25 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
     const float* w = a.weights + blockIdx.x * a.weight_stride;
     const uint32_t lo = a.first, hi = a.count - a.recent;  // the candidates
     uint32_t want = a.keep - a.first - a.recent;
-    const bool any = want > 0;
+    const bool any = want > 0, vec = (reinterpret_cast<uintptr_t>(w) & 15u) == 0;
     hist[tid >> 8][tid & 255] = 0;
 
     uint32_t key[kPer];
     float value[kPer];
     auto load = [&](uint32_t base) {
+        const uint32_t j0 = base + tid * kPer;
+        if (vec && j0 + kPer <= a.count) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const uint32_t j = base + tid * kPer + e;
-            value[e] = j < a.count ? w[j] : 0.0f;
+            for (int e = 0; e < kPer; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(w + j0 + e);
+                value[e] = x.x;
+                value[e + 1] = x.y;
+                value[e + 2] = x.z;
+                value[e + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) value[e] = j0 + e < a.count ? w[j0 + e] : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < kPer; ++e) key[e] = weight_key(value[e]);
@@ -232,12 +240,25 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
 #pragma unroll
         for (int pass = 0; pass < 4; ++pass) {
             const int shift = 24 - 8 * pass;
-            for (uint32_t base = 0; base < a.count; base += kStretch) {
-                if (!CACHED) load(base);
+            if constexpr (CACHED) {
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) {
-                    const uint32_t j = base + tid * kPer + e;
+                    const uint32_t j = tid * kPer + e;
                     if (j >= lo && j < hi && (key[e] & mask) == prefix) atomicAdd(&hist[pass][key[e] >> shift & 255], 1u);
+                }
+            } else {
+                // Counting asks for no order: lanes side by side.
+                for (uint32_t base = lo; base < hi; base += kStretch) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        const uint32_t j = base + e * kSelectThreads + tid;
+                        value[e] = j < hi ? w[j] : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) {
+                        const uint32_t k = weight_key(value[e]);
+                        if (base + e * kSelectThreads + tid < hi && (k & mask) == prefix) atomicAdd(&hist[pass][k >> shift & 255], 1u);
+                    }
                 }
             }
             __syncthreads();
@@ -584,10 +605,13 @@ extern "C" mhip_status mhip_kv_evict_mx4(mhip_ctx* ctx, const void* k_store, con
     sel.first = static_cast<uint32_t>(p->first);
     sel.recent = static_cast<uint32_t>(p->recent);
     sel.out_rows = static_cast<uint32_t>(out_shape->capacity);
-    if (p->key_count <= kSelectThreads * kSelectPer)
-        mhip::launch(ctx, mx4_select_kernel<true>, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, sel);
+    const dim3 grid(static_cast<unsigned>(rows)), block(kSelectThreads);
+    if (p->key_count <= kSelectThreads * 8)
+        mhip::launch(ctx, mx4_select_kernel<8, true>, grid, block, 0, sel);
+    else if (p->key_count <= kSelectThreads * 16)
+        mhip::launch(ctx, mx4_select_kernel<16, true>, grid, block, 0, sel);
     else
-        mhip::launch(ctx, mx4_select_kernel<false>, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, sel);
+        mhip::launch(ctx, mx4_select_kernel<16, false>, grid, block, 0, sel);
     st = mhip::check_launch("kv-evict (select)");
     if (st != MHIP_OK || p->keep == 0) return st;
 

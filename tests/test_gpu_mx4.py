@@ -313,6 +313,9 @@ def evict_case(dev, batch, heads, d, cap, count, keep, first, recent, weights, o
     (1, 1, 32, 8, 8, 3, 0, 0), (1, 2, 64, 10, 9, 9, 0, 0), (2, 3, 80, 101, 100, 37, 4, 10),
     (1, 2, 128, 2100, 2047, 1022, 4, 128), (1, 1, 256, 60, 60, 1, 0, 1), (1, 1, 33, 60, 60, 1, 1, 0),
     (1, 2, 64, 60, 60, 20, 8, 12), (1, 1, 64, 5000, 4999, 4097, 0, 0), (3, 2, 96, 300, 270, 0, 0, 0),
+    # On both sides of what a workgroup's registers hold.
+    (1, 1, 32, 8193, 8192, 5000, 3, 7), (1, 2, 32, 8200, 8193, 4100, 0, 100), (1, 1, 32, 16385, 16384, 9000, 0, 0), (1, 1, 32, 16387, 16385, 9000, 4, 500),
+    (1, 1, 32, 40000, 39999, 30001, 0, 0),
 ])
 def test_eviction_keeps_the_heaviest(dev, in_place, batch, heads, d, cap, count, keep, first, recent):
     rng = np.random.default_rng(cap)
@@ -324,6 +327,8 @@ def test_eviction_keeps_the_heaviest(dev, in_place, batch, heads, d, cap, count,
 def test_eviction_ties_and_odd_weights(dev, kind):
     """Ties go to the lowest row; NaN counts as -inf and -0 as 0."""
     rng = np.random.default_rng(8)
+    if kind == "few":  # ties across the stretches of a long account
+        evict_case(dev, 1, 1, 32, 33000, 32999, 20001, 5, 9, rng.integers(0, 3, (1, 1, 33000)).astype(np.float32))
     w = rng.integers(0, 3, (1, 2, 1500)).astype(np.float32)
     if kind == "equal":
         w[:] = 1.5
