@@ -921,7 +921,7 @@ __device__ __forceinline__ void tile_scores(const char* kt, const QPlanes<NB>& q
 __device__ __forceinline__ void copy_to_lds(const char* from, char* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(
         static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to)));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
 }
 
 // The words of a tile's NaN bits together.
@@ -1241,7 +1241,8 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
     // The rows whose queries admit a key of the workgroup, the chunk's share.
     const int off = a.kv - a.seq, last_key = min(first + kSumKeys, a.kv) - 1;
     const int i0 = a.causal ? max(0, first - off) : 0;
-    const int i1 = a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(a.seq), static_cast<int64_t>(last_key) - off + a.window)) : a.seq;
+    const int64_t past = static_cast<int64_t>(last_key) - off + a.window;  // a window's last query, and one
+    const int i1 = a.window > 0 ? static_cast<int>(max(min(static_cast<int64_t>(a.seq), past), static_cast<int64_t>(0))) : a.seq;
     const int begin = i0 * a.group / 32, end = max((i1 * a.group + 31) / 32, begin), per = (end - begin + chunks - 1) / chunks;
     const int r0 = min(begin + chunk * per, end), r1 = min(r0 + per, end);
     const char* planes = a.planes + pair * a.planes_ld * Cfg::kBytes;

@@ -541,3 +541,74 @@ def test_unaligned_rows_and_outputs(dev):
         got = into.numpy()
         assert got[0] == 0.0
         assert_bitexact(got[1:].reshape(q.shape), want)
+
+
+def test_weights_of_a_window_far_down_a_long_cache(dev):
+    """A window's rows are counted back from every key of the cache: 2.2 million
+    keys under 1024 query heads of one KV head pass 31 bits. Zeros are held, so
+    each of the 16 keys admitted gets 1/16 from each head, exactly."""
+    from magnetar_hip import ops
+    heads, d, kv, window = 1024, 32, 2200000, 16
+    k, v = (ops.Mx4Store(dev, kv, 1, d) for _ in range(2))
+    q = dev.upload(np.random.default_rng(3).standard_normal((1, heads * d)).astype(np.float32))
+    w = dev.zeros((1, 1, kv))
+    out = ops.attention_mx4(dev, q, k, v, ops.attention_params(1, kv, heads, d, kv_head_count=1, causal=True, window_size=window),
+                            weights=w, weights_out=w)
+    assert not out.numpy().any()
+    got = w.numpy()[0, 0]
+    assert not got[:-window].any() and (got[-window:] == heads / window).all()
+
+
+@pytest.mark.parametrize("seq,kv", [(1, 300), (5, 300), (60, 300), (600, 900)])
+def test_sequences_at_strides_of_their_own(dev, seq, kv):
+    """Queries, outputs and stores of a batch at strides of their own: the bits
+    of each sequence by itself, what lies between left alone; then an eviction
+    in place of the same stores."""
+    import ctypes
+
+    from magnetar_hip import _lib, ops
+    batch, heads, kv_heads, d, cap = 2, 4, 2, 64, kv + 5
+    one = kv_heads * -(-cap // 4) * 68 * 2
+    stride, q_bs, o_bs = one + (-one) % 16 + 32, seq * heads * d + 8, seq * heads * d + 4
+    rows = [[cache_rows(10 * i + b, kv, kv_heads, d) for b in range(batch)] for i in range(2)]
+    held = [dev.upload(np.full(batch * stride, 0xAB, np.uint8)) for _ in range(2)]
+    alone = [[store_of(dev, rows[i][b], cap, kv_heads, d) for b in range(batch)] for i in range(2)]
+    shape = _lib.Mx4StoreShape(cap, kv_heads, d, batch, stride)
+    for i in range(2):
+        both = dev.upload(np.stack(rows[i]))
+        _lib.call("mhip_kv_write_mx4", dev.ctx, ctypes.c_void_p(held[i].ptr), ctypes.byref(shape), ctypes.c_void_p(both.ptr), kv, 0)
+    q = np.random.default_rng(seq).standard_normal((batch, q_bs)).astype(np.float32)
+    x = dev.upload(q)
+    out, w = dev.upload(np.full((batch, o_bs), 5.0, np.float32)), dev.zeros((batch, kv_heads, cap))
+    p = ops.attention_params(seq, cap, heads, d, kv_head_count=kv_heads, causal=True, key_count=kv, batch=batch)
+    p.q_batch_stride, p.out_batch_stride, p.kv_batch_stride, p.v_batch_stride = q_bs, o_bs, stride, stride
+    _lib.call("mhip_attention_mx4", dev.ctx, *(ctypes.c_void_p(t.ptr) for t in (x, held[0], held[1], out)), ctypes.byref(p), None,
+              ctypes.c_void_p(w.ptr))
+    got, got_w = out.numpy(), w.numpy()
+    assert (got[:, seq * heads * d:] == 5.0).all()
+    for b in range(batch):
+        pb = ops.attention_params(seq, cap, heads, d, kv_head_count=kv_heads, causal=True, key_count=kv)
+        w1 = dev.zeros((1, kv_heads, cap))
+        want = ops.attention_mx4(dev, dev.upload(q[b, :seq * heads * d]), alone[0][b], alone[1][b], pb, weights_out=w1).numpy()
+        # One sequence's chunks may be shorter: the same sums in another order.
+        held_rows = [ref.round_trip(rows[i][b], kv_heads, d) for i in range(2)]
+        exact, received, largest = ref.attention(q[b, :seq * heads * d].reshape(seq, -1), *held_rows, heads, kv_heads, d)
+        tol = ref.attention_tolerance(d, largest)
+        assert rel(got[b, :seq * heads * d], want.ravel()) <= 2 * tol
+        assert rel(got[b, :seq * heads * d], exact.ravel()) <= tol
+        assert rel(got_w[b, :, :kv], received) <= tol and not got_w[b, :, kv:].any()
+    keep = kv // 2
+    e = _lib.KvEvictParams(kv, keep, 2, 9, cap, cap)
+    _lib.call("mhip_kv_evict_mx4", dev.ctx, ctypes.c_void_p(held[0].ptr), ctypes.c_void_p(held[1].ptr), ctypes.c_void_p(w.ptr),
+              ctypes.byref(shape), ctypes.byref(e), ctypes.c_void_p(held[0].ptr), ctypes.c_void_p(held[1].ptr), ctypes.byref(shape),
+              ctypes.c_void_p(w.ptr), None)
+    for i in range(2):
+        into = dev.zeros((batch, keep, kv_heads, d))
+        _lib.call("mhip_kv_read_mx4", dev.ctx, ctypes.c_void_p(held[i].ptr), ctypes.byref(shape), ctypes.c_void_p(into.ptr), keep, 0)
+        kept = into.numpy()
+        for b in range(batch):
+            full = ref.round_trip(rows[i][b], kv_heads, d).reshape(kv, kv_heads, d)
+            for h in range(kv_heads):
+                at = ref.evict(got_w[b, h], kv, keep, 2, 9)
+                assert np.array_equal(kept[b, :, h], full[at, h])
+        assert (held[i].numpy().reshape(batch, stride)[:, one:] == 0xAB).all()
