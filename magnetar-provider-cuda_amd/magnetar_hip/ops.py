@@ -260,6 +260,8 @@ def kv_evict_mx4(dev: Device, k: Mx4Store, v: Mx4Store, weights: DeviceArray, ke
         raise ValueError("kv-evict indices must be [batch, kv_heads, keep]")
     if k._key != v._key or k_out._key != v_out._key:
         raise ValueError("kv-evict: the key and the value store differ in shape")
+    if weights.shape[-1] < key_count or weights_out.shape[-1] < k_out._key[0]:
+        raise ValueError("kv-evict: weights for fewer rows than the stores have")
     p = _lib.KvEvictParams(key_count, keep, first, recent, weights.shape[-1], weights_out.shape[-1])
     call("mhip_kv_evict_mx4", dev.ctx, _p(k.data), _p(v.data), _p(weights), k._ref,
          ctypes.byref(p), _p(k_out.data), _p(v_out.data), k_out._ref, _p(weights_out), _p(indices))

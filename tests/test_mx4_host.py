@@ -147,3 +147,16 @@ def test_evict_refusals(mh, params, out, buffers, code, words):
     got, detail = _call(mh, "mhip_kv_evict_mx4", b[0], b[1], b[2], ctypes.byref(s), ctypes.byref(p), b[3],
                         b[4], ctypes.byref(o), b[5], None)
     assert got == code and words in detail, (got, detail)
+
+
+@pytest.mark.parametrize("count,width,width_out", [(60, 59, 64), (1, 0, 64), (60, 64, 63), (60, 64, 0)])
+def test_evict_refuses_weights_of_fewer_rows(mh, count, width, width_out):
+    """Before any call: weights of no rows would else pass as the stride 0, the
+    store's capacity."""
+    def array(*shape):
+        return mh.DeviceArray(None, 0, shape, np.float32, owned=False)
+
+    store = object.__new__(mh.ops.Mx4Store)
+    store._key = (64, 2, 32, 1)
+    with pytest.raises(ValueError, match="fewer rows"):
+        mh.ops.kv_evict_mx4(None, store, store, array(1, 2, width), count, 1, store, store, array(1, 2, width_out))
