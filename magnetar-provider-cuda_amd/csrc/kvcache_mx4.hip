@@ -390,9 +390,11 @@ __device__ __forceinline__ void take_row(const uint8_t* from, int r, uint32_t (&
 // Rows of `src` to rows 0 .. keep - 1 of `dst`: row indices[i], or i itself
 // where indices is null. 16 lanes a group of four rows, as for a write;
 // blockIdx.y: the keys' or the values' store. A kept row is 4 NB bytes of each of
-// its group's lines, so that the groups with a kept row are read whole: half the
-// rows of 2 x 36 MB in 18-23 us, 90 MB read and written. In place the rows go by
-// way of the workspace (another 20 us): a row may move across a workgroup's.
+// its group's lines, so that the groups with a kept row are read whole: 2050 of
+// 8192 rows of 64 heads of 128 in 19 us, about 44 MB of lines read and 18 written
+// (23 us with a row's loads after the last one's). In place
+// the rows go by way of the workspace, a second launch: they may move across
+// workgroups.
 struct MoveArgs {
     StoreArgs src[2], dst[2];
     const uint32_t* indices;
@@ -407,16 +409,21 @@ __global__ __launch_bounds__(256) void mx4_move_kernel(MoveArgs a) {
     const uint32_t group = u % a.groups_touched, bh = u / a.groups_touched;
     const uint32_t h = bh % dst.heads, b = bh / dst.heads;
     const int hi = static_cast<int>(min(4u, a.keep - group * 4));
-    uint32_t code[NB];
+    uint32_t code[NB], row[4];
     uint32_t scale = 0;  // of block p = n
 #pragma unroll
     for (int p = 0; p < NB; ++p) code[p] = 0;
+    // A last group's rows past `keep` are read as its last one, and not written.
+#pragma unroll
+    for (int r = 0; r < 4; ++r) row[r] = group * 4 + min(r, hi - 1);
+    if (a.indices)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) row[r] = a.indices[static_cast<uint64_t>(bh) * a.keep + row[r]];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        if (r >= hi) continue;
-        const uint32_t row = a.indices ? a.indices[static_cast<uint64_t>(bh) * a.keep + group * 4 + r] : group * 4 + r;
-        take_row<NB>(unit_ptr<NB>(src, b, h, row / 4, n) + (row % 4) * NB, r, code);
-        if (n < NB) scale |= static_cast<uint32_t>(scale_ptr<NB>(src, b, h, row / 4)[4 * n + row % 4]) << (8 * r);
+        take_row<NB>(unit_ptr<NB>(src, b, h, row[r] / 4, n) + (row[r] % 4) * NB, r, code);
+        const uint32_t x = scale_ptr<NB>(src, b, h, row[r] / 4)[4 * min(n, NB - 1u) + row[r] % 4];
+        scale |= x << (8 * r);
     }
     uint8_t* to = unit_ptr<NB>(dst, b, h, group, n);
     uint8_t* sto = scale_ptr<NB>(dst, b, h, group) + 4 * n;
