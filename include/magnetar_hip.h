@@ -322,7 +322,8 @@ uint64_t mhip_kv_mx4_bytes(uint64_t capacity, uint64_t kv_heads, uint64_t head_d
 mhip_status mhip_kv_write_mx4(mhip_ctx* ctx, void* store, const mhip_mx4_store* shape,
                               const float* rows, uint64_t count, uint64_t row_offset);
 /* The values that rows [row_offset, row_offset + count) of each store hold,
- * to rows [batch][count, kv_heads * head_dimension]. */
+ * to rows [batch][count, kv_heads * head_dimension]. Nothing advances in a
+ * captured step. */
 mhip_status mhip_kv_read_mx4(mhip_ctx* ctx, const void* store, const mhip_mx4_store* shape,
                              float* rows, uint64_t count, uint64_t row_offset);
 /* mhip_attention_f32 over a key and a value store of kv_rows rows: the same
@@ -332,7 +333,8 @@ mhip_status mhip_kv_read_mx4(mhip_ctx* ctx, const void* store, const mhip_mx4_st
  * weights_out = weights + the sum, over the queries and the query heads of the
  * KV head, of the softmax weight given to the key, for the kv_seq_len keys in
  * use; entries past them stay as they are. weights has the same layout, NULL
- * counts as zeros, and may be weights_out itself. */
+ * counts as zeros, and may be weights_out itself. A call that asks for them has
+ * a query (seq_len above 0). */
 mhip_status mhip_attention_mx4(mhip_ctx* ctx, const float* q, const void* k_store,
                                const void* v_store, float* out,
                                const mhip_attention_params* params, const float* weights,

@@ -16,9 +16,10 @@
 // rounded up to 256 bytes. Byte (n, row, p) holds the codes of the head's
 // values 32 p + n (low four bits) and 32 p + 16 + n (high): the two share a
 // scale, which one conversion takes. A unit (head, group, n) is NB dwords with
-// all four rows of its 2 NB columns, and both products of attention are fed
-// from whole units, with no pass through LDS (attention_mx4.hip). A head's
-// rows are contiguous, so a chunk of keys is one stretch of memory.
+// all four rows of its 2 NB columns, and for a token's few rows both products of
+// attention are fed from whole units, with no pass through LDS
+// (attention_mx4.hip). A head's rows are contiguous, so a chunk of keys is one
+// stretch of memory.
 #pragma once
 
 #include "common.hpp"
