@@ -805,6 +805,18 @@ struct SumCfg {
     static constexpr int kBytes = (kSteps * (kQPlanes * kPlaneBytes + 512) + 1023) / 1024 * 1024;
 };
 
+template <int NB>
+__device__ __forceinline__ void keep_planes(const Mx4Attn& a, int b, int kvh, int tile, const QPlanes<NB>& q) {
+    const int lane = threadIdx.x & 63;
+    char* to = a.planes + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.planes_ld + tile) * SumCfg<NB>::kBytes;
+#pragma unroll
+    for (int s = 0; s < QPlanes<NB>::kSteps; ++s) {
+#pragma unroll
+        for (int n = 0; n < kQPlanes; ++n) store_plane(to + (s * kQPlanes + n) * kPlaneBytes + lane * 16, q.f[s][n]);
+        *reinterpret_cast<uint2*>(to + QPlanes<NB>::kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8) = uint2{q.scale[s][0], q.scale[s][1]};
+    }
+}
+
 // What a thread carries from memory to LDS: a unit of each store with its scales.
 template <int NB>
 struct Carry {
@@ -1007,6 +1019,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, NB > 4 ? 1 : 2) void mx4_prompt_
     __syncthreads();
     QPlanes<NB> qp;
     make_q_planes<NB>(wrows + q * Cfg::kRow, h, qp);
+    if (a.planes && at.chunk == 0 && wave_live) keep_planes<NB>(a, b, kvh, at.row0 / 32 + wave, qp);
     __syncthreads();
     char* low = lds + 2 * Cfg::kBytes + wave * Cfg::kLowBytes + lane * 16;
     if constexpr (QPlanes<NB>::kLow)
@@ -1224,13 +1237,7 @@ __global__ __launch_bounds__(64) void mx4_planes_kernel(Mx4Attn a) {
     __syncthreads();
     QPlanes<NB> q;
     make_q_planes<NB>(rows + (lane & 31) * kRow, lane >> 5, q);
-    char* to = a.planes + ((static_cast<uint64_t>(b) * a.kv_heads + kvh) * a.planes_ld + tile) * SumCfg<NB>::kBytes;
-#pragma unroll
-    for (int s = 0; s < QPlanes<NB>::kSteps; ++s) {
-#pragma unroll
-        for (int n = 0; n < kQPlanes; ++n) store_plane(to + (s * kQPlanes + n) * kPlaneBytes + lane * 16, q.f[s][n]);
-        *reinterpret_cast<uint2*>(to + QPlanes<NB>::kSteps * kQPlanes * kPlaneBytes + s * 512 + lane * 8) = uint2{q.scale[s][0], q.scale[s][1]};
-    }
+    keep_planes<NB>(a, b, kvh, tile, q);
 }
 
 // The attention each key received from any number of rows, the scores taken
@@ -1253,11 +1260,11 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
     __shared__ __attribute__((aligned(16))) char lds[2][Cfg::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 31, h = lane >> 5;
-    const int kvh = blockIdx.y, b = blockIdx.z;
-    const int block = chunks > 1 ? blockIdx.x / chunks : blockIdx.x, chunk = chunks > 1 ? blockIdx.x % chunks : 0;
+    const int pairs = a.kv_heads * a.batch, unit = blockIdx.x / pairs, pair = blockIdx.x - unit * pairs;
+    const int b = pair / a.kv_heads, kvh = pair - b * a.kv_heads;
+    const int block = unit / chunks, chunk = unit - block * chunks;
     const int first = block * kSumKeys, base = first + wave * 64;
     if (first >= a.kv) return;
-    const uint64_t pair = static_cast<uint64_t>(b) * a.kv_heads + kvh;
 
     // The rows whose queries admit a key of the workgroup, the chunk's share.
     const int off = a.kv - a.seq, last_key = min(first + kSumKeys, a.kv) - 1;
@@ -1266,7 +1273,7 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
     const int i1 = a.window > 0 ? static_cast<int>(max(min(static_cast<int64_t>(a.seq), past), static_cast<int64_t>(0))) : a.seq;
     const int begin = i0 * a.group / 32, end = max((i1 * a.group + 31) / 32, begin), per = (end - begin + chunks - 1) / chunks;
     const int r0 = min(begin + chunk * per, end), r1 = min(r0 + per, end);
-    const char* planes = a.planes + pair * a.planes_ld * Cfg::kBytes;
+    const char* planes = a.planes + static_cast<uint64_t>(pair) * a.planes_ld * Cfg::kBytes;
     auto fetch = [&](int t) {
         const char* from = planes + static_cast<uint64_t>(t) * Cfg::kBytes;
 #pragma unroll
@@ -1301,7 +1308,7 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
             kscale[kk][s / 2] |= (2 * s + h < NB ? static_cast<uint32_t>(sc[4 * p]) : 127u) << (16 * (s % 2));
         }
     }
-    const float* stats = a.stats + pair * a.rows * 2;
+    const float* stats = a.stats + static_cast<uint64_t>(pair) * a.rows * 2;
     float sum[2][16] = {};
     auto row_stats = [&](int t) { return *reinterpret_cast<const f32x2*>(stats + 2 * min(32 * t + m, a.rows - 1)); };
     f32x2 next = row_stats(r0);
@@ -1369,9 +1376,10 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
             const int key = base + 32 * kk + 8 * (e / 4) + 4 * h + e % 4;
             if (key >= a.kv) continue;
             if (chunks > 1)
-                part[(pair * chunks + chunk) * part_ld + key] = sum[kk][e];
+                part[(static_cast<uint64_t>(pair) * chunks + chunk) * part_ld + key] = sum[kk][e];
             else
-                weights_out[pair * stride + key] = (weights ? weights[pair * stride + key] : 0.0f) + sum[kk][e];
+                weights_out[static_cast<uint64_t>(pair) * stride + key] =
+                    (weights ? weights[static_cast<uint64_t>(pair) * stride + key] : 0.0f) + sum[kk][e];
         }
 }
 
@@ -1424,12 +1432,13 @@ SumPlan sum_plan(mhip_ctx* ctx, Mx4Attn& a, uint64_t pairs, uint64_t kv_rows) {
     return p;
 }
 template <int NB>
-mhip_status launch_weights(mhip_ctx* ctx, const Mx4Attn& a, uint64_t batch, const SumPlan& p, float* part, const float* weights,
-                           float* weights_out, uint64_t stride) {
+mhip_status launch_weights(mhip_ctx* ctx, const Mx4Attn& a, uint64_t batch, bool planes, const SumPlan& p, float* part,
+                           const float* weights, float* weights_out, uint64_t stride) {
     const dim3 heads(1, static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch));
-    if (p.key_blocks * p.chunks * kPromptWaves * 64 >= (1ULL << 32)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
-    mhip::launch(ctx, mx4_planes_kernel<NB>, dim3(static_cast<unsigned>(a.planes_ld), heads.y, heads.z), dim3(64), 0, a);
-    mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(p.key_blocks * p.chunks), heads.y, heads.z),
+    const uint64_t blocks = p.key_blocks * p.chunks * a.kv_heads * batch;
+    if (blocks * kPromptWaves * 64 >= (1ULL << 32)) return mhip::fail(MHIP_SHAPE_UNSUPPORTED, "attention: too many rows");
+    if (!planes) mhip::launch(ctx, mx4_planes_kernel<NB>, dim3(static_cast<unsigned>(a.planes_ld), heads.y, heads.z), dim3(64), 0, a);
+    mhip::launch(ctx, mx4_weights_kernel<NB>, dim3(static_cast<unsigned>(blocks)),
                  dim3(64 * kPromptWaves), 0, a, weights, weights_out, stride, static_cast<int>(p.chunks), part, p.keys);
     if (p.chunks > 1)
         mhip::launch(ctx, mx4_sum_weights_kernel, dim3(static_cast<unsigned>(mhip::ceil_div(p.keys, 256)), heads.y, heads.z), dim3(256), 0,
@@ -1441,6 +1450,7 @@ template <int NB, bool FEW>
 mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* weights, float* weights_out,
                         uint64_t stride, uint64_t kv_rows) {
     a.row_tiles = static_cast<int>(mhip::ceil_div(a.rows, kRowTile<FEW>));
+    a.batch = static_cast<int>(batch);
     const uint64_t tiles = batch * a.kv_heads * a.row_tiles;
     // A workgroup for each CU, of at least a strip a wave. (Two on each, with half
     // the chunk: 8 x 4096 keys 19 us for 15, 131073 keys 42 for 33, what the
@@ -1478,7 +1488,7 @@ mhip_status launch_rows(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float* 
     mhip::launch(ctx, mx4_rows_kernel<NB, FEW>, grid, dim3(64 * kRowWaves<NB>), 0, a);
     mhip_status st = mhip::check_launch("attention (4-bit)");
     if (st != MHIP_OK || !weights_out) return st;
-    if (!keep) return launch_weights<NB>(ctx, a, batch, sums, part, weights, weights_out, stride);
+    if (!keep) return launch_weights<NB>(ctx, a, batch, false, sums, part, weights, weights_out, stride);
     const uint64_t keys = a.advance ? kv_rows : static_cast<uint64_t>(a.kv);
     mhip::launch(ctx, mx4_kept_weights_kernel,
                  dim3(static_cast<unsigned>(mhip::ceil_div(keys, 1024)), static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(batch)),
@@ -1518,7 +1528,7 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
         mhip_status st = mhip::workspace(ctx, bytes, &ws);
         if (st != MHIP_OK) return st;
         char* at = static_cast<char*>(ws);
-        a.planes = at;
+        a.planes = weights_out ? at : nullptr;
         a.part_o = reinterpret_cast<float*>(at += sums.plane_bytes);
         a.part_ml = a.part_o + records * (32 * NB);
         part = reinterpret_cast<float*>(at += record_bytes);
@@ -1534,7 +1544,7 @@ mhip_status launch_prompt(mhip_ctx* ctx, Mx4Attn& a, uint64_t batch, const float
         st = mhip::check_launch("attention (4-bit, prompt merge)");
     }
     if (st != MHIP_OK || !weights_out) return st;
-    return launch_weights<NB>(ctx, a, batch, sums, part, weights, weights_out, stride);
+    return launch_weights<NB>(ctx, a, batch, true, sums, part, weights, weights_out, stride);
 }
 
 // Which of the two attention kernels is the faster one, in microseconds of time

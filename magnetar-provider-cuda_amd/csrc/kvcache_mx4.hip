@@ -207,11 +207,24 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// The sum over the lanes up to this one, in the registers of a wave: shifts
+// within rows of 16, then the rows' and the halves' last sums passed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+    v = add_dpp<0x118, 0xF>(add_dpp<0x114, 0xF>(add_dpp<0x112, 0xF>(add_dpp<0x111, 0xF>(v))));  // row_shr
+    return add_dpp<0x143, 0xC>(add_dpp<0x142, 0xA>(v));  // row_bcast:15, row_bcast:31
+}
+
 // One workgroup per (sequence, head). The threshold weight is found by its
 // bytes, the highest first: a histogram in LDS of the candidates that match
 // the bytes found so far, its running count from the top taken by every wave
-// for itself, so that a byte costs one barrier. Then, in one scan, the rows
-// above the threshold and the first ones at it, in order.
+// for itself, so that a byte costs one barrier. Weights have few first bytes
+// (their signs and exponents), at which a wave's lanes would queue: that
+// histogram is eight, a lane's by its number. Then, in one scan, the rows above
+// the threshold and the first ones at it, in order.
 //
 // A thread has kPer rows side by side. Up to 16 * 1024 rows (CACHED) their keys
 // stay in its registers over the five passes, 8 or 16 a thread; longer accounts
@@ -220,14 +233,18 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 template <int kPer, bool CACHED>
 __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a) {
     constexpr uint32_t kStretch = kPer * kSelectThreads;
-    __shared__ uint32_t hist[4][256];
+    constexpr int kCopies = 8;
+    __shared__ __attribute__((aligned(16))) uint32_t hist0[256][kCopies];
+    __shared__ uint32_t hist[3][256];
     __shared__ uint32_t wave_above[kSelectThreads / 64], wave_equal[kSelectThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* w = a.weights + blockIdx.x * a.weight_stride;
     const uint32_t lo = a.first, hi = a.count - a.recent;  // the candidates
     uint32_t want = a.keep - a.first - a.recent;
     const bool any = want > 0, vec = (reinterpret_cast<uintptr_t>(w) & 15u) == 0;
-    hist[tid >> 8][tid & 255] = 0;
+    (&hist0[0][0])[tid] = (&hist0[0][0])[tid + kSelectThreads] = 0;
+    if (tid < 3 * 256) (&hist[0][0])[tid] = 0;
+    auto count = [&](int pass, uint32_t byte) { atomicAdd(pass == 0 ? &hist0[byte][lane % kCopies] : &hist[pass - 1][byte], 1u); };
 
     uint32_t key[kPer];
     float value[kPer];
@@ -260,7 +277,7 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) {
                     const uint32_t j = tid * kPer + e;
-                    if (j >= lo && j < hi && (key[e] & mask) == prefix) atomicAdd(&hist[pass][key[e] >> shift & 255], 1u);
+                    if (j >= lo && j < hi && (key[e] & mask) == prefix) count(pass, key[e] >> shift & 255);
                 }
             } else {
                 // Counting asks for no order: lanes side by side.
@@ -273,7 +290,7 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
 #pragma unroll
                     for (int e = 0; e < kPer; ++e) {
                         const uint32_t k = weight_key(value[e]);
-                        if (base + e * kSelectThreads + tid < hi && (k & mask) == prefix) atomicAdd(&hist[pass][k >> shift & 255], 1u);
+                        if (base + e * kSelectThreads + tid < hi && (k & mask) == prefix) count(pass, k >> shift & 255);
                     }
                 }
             }
@@ -283,15 +300,16 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
             uint32_t bin[4], mine = 0;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                bin[x] = hist[pass][255 - 4 * lane - x];
+                const int byte = 255 - 4 * lane - x;
+                if (pass == 0) {
+                    const uint4* c = reinterpret_cast<const uint4*>(hist0[byte]);
+                    bin[x] = c[0].x + c[0].y + c[0].z + c[0].w + c[1].x + c[1].y + c[1].z + c[1].w;
+                } else {
+                    bin[x] = hist[pass - 1][byte];
+                }
                 mine += bin[x];
             }
-            uint32_t upto = mine;
-#pragma unroll
-            for (int off = 1; off < 64; off *= 2) {
-                const uint32_t v = static_cast<uint32_t>(__shfl_up(static_cast<int>(upto), off, 64));
-                if (lane >= off) upto += v;
-            }
+            const uint32_t upto = scan64(mine);
             const int at = __ffsll(static_cast<unsigned long long>(__ballot(upto >= want))) - 1;
             uint32_t left = want - (upto - mine), byte = 255 - 4 * lane;
 #pragma unroll
@@ -300,8 +318,8 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
                     left -= bin[x];
                     --byte;
                 }
-            want = static_cast<uint32_t>(__shfl(static_cast<int>(left), at, 64));
-            prefix |= static_cast<uint32_t>(__shfl(static_cast<int>(byte), at, 64)) << shift;
+            want = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(left), at));
+            prefix |= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(byte), at)) << shift;
             mask |= 255u << shift;
         }
     }
@@ -320,17 +338,8 @@ __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a
                 if (!forced && any && key[e] == prefix) equal |= 1u << e;
             }
         }
-        uint32_t na = static_cast<uint32_t>(__popc(above)), ne = static_cast<uint32_t>(__popc(equal));
-        const uint32_t own_a = na, own_e = ne;
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) {
-            const uint32_t va = static_cast<uint32_t>(__shfl_up(static_cast<int>(na), off, 64));
-            const uint32_t ve = static_cast<uint32_t>(__shfl_up(static_cast<int>(ne), off, 64));
-            if (lane >= off) {
-                na += va;
-                ne += ve;
-            }
-        }
+        const uint32_t own_a = static_cast<uint32_t>(__popc(above)), own_e = static_cast<uint32_t>(__popc(equal));
+        uint32_t na = scan64(own_a), ne = scan64(own_e);
         if (lane == 63) {
             wave_above[wave] = na;
             wave_equal[wave] = ne;
