@@ -1295,6 +1295,10 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
         const uint64_t g = static_cast<uint64_t>(kvh) * a.groups + key / 4;
         const uint8_t* unit = ks + g * 64 * NB + (key % 4) * NB;
         const uint8_t* sc = ks + a.code_bytes + g * 4 * NB + key % 4;
+        uint32_t four[16];  // heads of four blocks: a key's four bytes of each unit
+        if constexpr (NB == 4)
+#pragma unroll
+            for (int n = 0; n < 16; ++n) four[n] = reinterpret_cast<const uint32_t*>(unit)[4 * n];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int p = min(2 * s + h, NB - 1);
@@ -1302,14 +1306,19 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
             for (int i = 0; i < 4; ++i) {
                 uint32_t w = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w |= static_cast<uint32_t>(unit[(4 * i + e) * 4 * NB + p]) << (8 * e);
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (NB == 4)
+                        w |= (four[4 * i + e] >> (8 * p) & 255u) << (8 * e);
+                    else
+                        w |= static_cast<uint32_t>(unit[(4 * i + e) * 4 * NB + p]) << (8 * e);
+                }
                 k[kk][s].u[i] = w;
             }
             kscale[kk][s / 2] |= (2 * s + h < NB ? static_cast<uint32_t>(sc[4 * p]) : 127u) << (16 * (s % 2));
         }
     }
     const float* stats = a.stats + static_cast<uint64_t>(pair) * a.rows * 2;
-    float sum[2][16] = {};
+    float sum[2][16] = {};  // [half of 32 keys][register of a product]
     auto row_stats = [&](int t) { return *reinterpret_cast<const f32x2*>(stats + 2 * min(32 * t + m, a.rows - 1)); };
     f32x2 next = row_stats(r0);
     for (int t = r0; t < r1; ++t) {
@@ -1362,25 +1371,24 @@ __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn 
                 }
         }
     }
+    // 32 keys' sums over 32 lanes: a lane passes on the half that is not its own,
+    // and has key m of them at the end.
+    float* v = &sum[0][0];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int d = 16; d > 0; d /= 2)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) sum[kk][e] += __shfl_xor(sum[kk][e], d, 64);
-    if (m != 0) return;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int key = base + 32 * kk + 8 * (e / 4) + 4 * h + e % 4;
-            if (key >= a.kv) continue;
-            if (chunks > 1)
-                part[(static_cast<uint64_t>(pair) * chunks + chunk) * part_ld + key] = sum[kk][e];
-            else
-                weights_out[static_cast<uint64_t>(pair) * stride + key] =
-                    (weights ? weights[static_cast<uint64_t>(pair) * stride + key] : 0.0f) + sum[kk][e];
+        for (int j = 0; j < d; ++j) {
+            const float keep = m & d ? v[j + d] : v[j], pass = m & d ? v[j] : v[j + d];
+            v[j] = keep + __shfl_xor(pass, d, 64);
         }
+    const int key = base + 32 * (m / 16) + 8 * (m % 16 / 4) + 4 * h + m % 4;
+    if (key >= a.kv) return;
+    if (chunks > 1) {
+        part[(static_cast<uint64_t>(pair) * chunks + chunk) * part_ld + key] = v[0];
+    } else {
+        const uint64_t at = static_cast<uint64_t>(pair) * stride + key;
+        weights_out[at] = (weights ? weights[at] : 0.0f) + v[0];
+    }
 }
 
 // The chunks' sums of a key, in their order.
