@@ -1222,8 +1222,9 @@ __global__ __launch_bounds__(256) void mx4_kept_weights_kernel(Mx4Attn a, const 
         if (key + x < kv) weights_out[at + x] = (weights ? weights[at + x] : 0.0f) + sum[x];
 }
 
-// The planes of Q for the weights' kernel: a wave 32 rows, by way of LDS. 13 us
-// for 1021 queries of 32 heads of 128, 17 MB read and 20 written.
+// The planes of Q for the weights' kernel where the rows kernel took the call (the
+// prompts' kernel keeps its own): a wave 32 rows, by way of LDS. 13 us for 1021
+// queries of 32 heads of 128, 17 MB read and 20 written.
 template <int NB>
 __global__ __launch_bounds__(64) void mx4_planes_kernel(Mx4Attn a) {
     constexpr int DP = 32 * NB, kRow = PromptCfg<NB>::kRow;
@@ -1244,11 +1245,14 @@ __global__ __launch_bounds__(64) void mx4_planes_kernel(Mx4Attn a) {
 // again by the prompts' scaled products from the planes of Q and the statistics
 // that the attention left: a wave holds 64 keys and walks the tiles of 32 rows
 // that admit one of the workgroup's (its share of them, of `chunks`), whose
-// planes the four waves share in LDS. The rows are the products' columns: a lane's sums are its
-// keys' over one column, and the columns are added up at the end, in a fixed
-// order; so are the chunks' sums, by mx4_sum_weights_kernel. 37 us and 5 for the
+// planes the four waves share in LDS. The rows are the products' columns: a lane's
+// sums are its keys' over one column, and the columns are added up at the end, in
+// a fixed order; so are the chunks' sums, by mx4_sum_weights_kernel. 20 us and 5 for the
 // sums beside an attention of 54 (1021 queries of 32 heads of 128 over as many
-// keys).
+// keys). A KV head's workgroups are `pairs` apart in the grid, on one XCD where
+// the heads are a multiple of eight, whose L2 then holds the head's planes (37 us for
+// 32 with neighbours in the grid); the last 12 were K's codes read by bytes and
+// the lanes' sums added up one key at a time.
 constexpr int kSumKeys = 64 * kPromptWaves, kSumRows = 8;
 template <int NB>
 __global__ __launch_bounds__(64 * kPromptWaves) void mx4_weights_kernel(Mx4Attn a, const float* __restrict__ weights,

@@ -229,7 +229,7 @@ __device__ __forceinline__ uint32_t scan64(uint32_t v) {
 // A thread has kPer rows side by side. Up to 16 * 1024 rows (CACHED) their keys
 // stay in its registers over the five passes, 8 or 16 a thread; longer accounts
 // are read again, stretch by stretch. What it waits for is latency: 8 x 8
-// accounts of 8192 weights 15 us, 2 MB.
+// accounts of 8192 weights 13.5 us, 2 MB.
 template <int kPer, bool CACHED>
 __global__ __launch_bounds__(kSelectThreads) void mx4_select_kernel(SelectArgs a) {
     constexpr uint32_t kStretch = kPer * kSelectThreads;
@@ -401,9 +401,8 @@ __device__ __forceinline__ void take_row(const uint8_t* from, int r, uint32_t (&
 // blockIdx.y: the keys' or the values' store. A kept row is 4 NB bytes of each of
 // its group's lines, so that the groups with a kept row are read whole: 2050 of
 // 8192 rows of 64 heads of 128 in 19 us, about 44 MB of lines read and 18 written
-// (23 us with a row's loads after the last one's). In place
-// the rows go by way of the workspace, a second launch: they may move across
-// workgroups.
+// (23 us with a row's loads after the last one's). In place the rows go by way of
+// the workspace, a second launch: they may move across workgroups.
 struct MoveArgs {
     StoreArgs src[2], dst[2];
     const uint32_t* indices;
